@@ -13,7 +13,8 @@
  *  - Matrices follow GGML order: a weight has `cols` = ne0 (the contraction
  *    dimension K) and `rows` = ne1.  Batched activations are x[b*cols + c],
  *    outputs y[b*rows + r] (the reference's layout, src/gguf_kernels.cpp:257).
- *  - GGML type ids: 0 F32, 1 F16, 2 Q4_0, 8 Q8_0, 14 Q6_K.
+ *  - GGML type ids: 0 F32, 1 F16, 2 Q4_0, 8 Q8_0, 14 Q6_K; activations of the
+ *    rotary, append and 4-bit attention calls also 30 BF16.
  *
  * Reference citations are path:line inside the MemVanta project.
  */
@@ -47,6 +48,7 @@ extern "C" {
 #define MV_TYPE_Q4_0 2
 #define MV_TYPE_Q8_0 8
 #define MV_TYPE_Q6_K 14
+#define MV_TYPE_BF16 30 /* activations of mv_rope_apply, mv_rope_kv_append, mv_kv_read, mv_paged_attn_q4* only */
 
 /* activation modes for mv_gemm (tensor_matmul_batch_v06) */
 #define MV_ACT_F32 0  /* fp32 activations: the reference's default prefill (src/gguf_kernels.cpp:268)            */
@@ -57,6 +59,16 @@ extern "C" {
 #define MV_KV_F16 1
 #define MV_KV_Q8 2    /* one fp32 scale per token over kv_dim (src/llama_model.cpp:22)                            */
 #define MV_KV_Q8_0 3  /* one fp32 scale per 32-element block (extension; no reference counterpart)               */
+#define MV_KV_Q4_0 4  /* 4 bits per value, one bf16 scale per 32-element block (extension; see mv_rope_kv_append) */
+
+/* pairs of a rotary position: (i, i + rot_dim/2) or (2i, 2i + 1) */
+#define MV_ROPE_HALF 0
+#define MV_ROPE_INTERLEAVED 1
+/* scaling of the rotary frequencies for contexts longer than the trained one (mv_rope_table) */
+#define MV_ROPE_SCALE_NONE 0
+#define MV_ROPE_SCALE_LINEAR 1 /* every frequency / factor                                                        */
+#define MV_ROPE_SCALE_YARN 2   /* by dimension: kept above beta_fast turns, / factor below beta_slow, ramp between */
+#define MV_ROPE_SCALE_BANDS 3  /* by turns: kept from beta_fast, / factor to beta_slow, linear in the turns between */
 
 typedef struct mv_weight_s* mv_weight_t;
 typedef struct mv_model_s* mv_model_t;
@@ -233,6 +245,96 @@ MV_API int mv_paged_attn_prefill(int kv_type, const float* q_dev, uint64_t n_q, 
                           const float* k_scales_dev, const float* v_scales_dev, const int32_t* block_table_dev,
                           uint64_t max_pages, uint64_t page, const int32_t* ctx_len_dev, uint64_t max_ctx,
                           float* out_dev, void* stream);
+
+/* ------------------------- rotary positions and the 4-bit cache (device) */
+
+/* cos and sin of position * frequency, [n_pos][rot_dim/2] fp32 each, computed
+ * in double and rounded once.  Frequency i is theta^(-2i/rot_dim), divided by
+ * freq_factors_dev[i] when that is given (GGUF rope_freqs.weight), then scaled:
+ * orig_ctx, beta_fast and beta_slow belong to YARN and BANDS (turns over
+ * orig_ctx positions), attn_factor to YARN: it multiplies cos and sin, 0 takes
+ * 0.1 ln(factor) + 1.  Extends the reference's unscaled tables
+ * (src/llama_model.cpp:233). */
+MV_API int mv_rope_table(uint64_t rot_dim, uint64_t n_pos, double theta, int scaling, double factor, double orig_ctx,
+                         double beta_fast, double beta_slow, double attn_factor, const float* freq_factors_dev,
+                         float* cos_dev, float* sin_dev, void* stream);
+
+/* Rotates the first rot_dim dimensions of every head of x by its row's
+ * position; the other dimensions are copied.  Head h of row r lies at
+ * x + r*x_row_stride + h*x_head_stride (elements, the head's own dimensions
+ * next to one another); out likewise, and out may be x with the same strides
+ * (other overlaps are not allowed).  type is MV_TYPE_F32, F16 or BF16.
+ * cos/sin as mv_rope_table writes them.  A row whose position is negative or
+ * >= n_pos gives zeros.  Extends mv_rope (src/llama_model.cpp:238), whose bits
+ * it gives for the half layout over whole F32 heads. */
+MV_API int mv_rope_apply(int type, const void* x_dev, uint64_t x_row_stride, uint64_t x_head_stride, void* out_dev,
+                         uint64_t out_row_stride, uint64_t out_head_stride, uint64_t rows, uint64_t n_head,
+                         uint64_t head_dim, uint64_t rot_dim, int layout, const float* cos_dev, const float* sin_dev,
+                         uint64_t n_pos, const int32_t* pos_dev, void* stream);
+
+/* mv_rope_apply on q (q_dev -> q_out_dev; n_head 0: no q) and k, and the append of the
+ * rotated k and of v to the paged cache, in one launch.  Row r is position
+ * pos[r] of sequence seq[r] (seq_dev NULL: sequence 0), page
+ * block_table[seq*max_pages + pos/page] of n_pages, slot pos%page.  rot_dim 0
+ * appends without rotation (cos/sin may be NULL).  Rows are skipped -- nothing is stored, q_out
+ * as in mv_rope_apply -- when the position is negative, not below n_pos
+ * (rot_dim > 0) or max_pages*page, or when the sequence or its page does not exist.  No two
+ * rows of a call may name the same slot.
+ * kv_type: every MV_KV_*, the pages and scales of mv_kv_append for the first
+ * four; F16 values are rounded to nearest even (mv_kv_append keeps the
+ * reference's conversion, which rounds ties up and loses a carry into an odd
+ * exponent: 1.9999 becomes 1).  MV_KV_Q4_0: k_pages / v_pages hold
+ * [n_pages][n_head_kv][page][head_dim/2] bytes, k_scales / v_scales
+ * [n_pages][n_head_kv][page][head_dim/32] bf16 (16-byte aligned, head_dim a
+ * multiple of 32).  A token's 32-bit words are ordered [4][head_dim/32]: word (t, b)
+ * holds dimensions 32b+8t .. +7, lowest nibble first.  A block of 32: mx its
+ * element of largest magnitude (first of equals), d = bf16(mx/-8), n =
+ * clamp(floor(x*(1/d) + 8.5), 0, 15), value (n-8)*d; a block with a NaN or
+ * infinity reads back as NaN.
+ * Replaces mv_rope + mv_kv_append (src/llama_model.cpp:238, :22). */
+MV_API int mv_rope_kv_append(int kv_type, int type, const void* q_dev, uint64_t q_row_stride, uint64_t q_head_stride,
+                             void* q_out_dev, uint64_t q_out_row_stride, uint64_t q_out_head_stride, uint64_t n_head,
+                             const void* k_dev, uint64_t k_row_stride, uint64_t k_head_stride, const void* v_dev,
+                             uint64_t v_row_stride, uint64_t v_head_stride, uint64_t n_head_kv, uint64_t rows,
+                             uint64_t head_dim, uint64_t rot_dim, int layout, const float* cos_dev,
+                             const float* sin_dev, uint64_t n_pos, const int32_t* seq_dev, const int32_t* pos_dev,
+                             const int32_t* block_table_dev, uint64_t n_seq, uint64_t max_pages, uint64_t page,
+                             uint64_t n_pages, void* k_pages_dev, void* v_pages_dev, void* k_scales_dev,
+                             void* v_scales_dev, void* stream);
+
+/* Rows of one pool of a paged cache (any MV_KV_*) as the values they stand for:
+ * out[rows][n_head_kv][head_dim] of out_type F32, F16 or BF16.  Rows are named
+ * as in mv_rope_kv_append; one that it would skip reads zeros. */
+MV_API int mv_kv_read(int kv_type, const void* pages_dev, const void* scales_dev, uint64_t n_head_kv,
+                      uint64_t head_dim, uint64_t rows, const int32_t* seq_dev, const int32_t* pos_dev,
+                      const int32_t* block_table_dev, uint64_t n_seq, uint64_t max_pages, uint64_t page,
+                      uint64_t n_pages, int out_type, void* out_dev, void* stream);
+
+/* Attention over an MV_KV_Q4_0 cache: one query row per sequence (row i is
+ * sequence i of the block table [n_seq][max_pages]) and its first ctx_len[i] tokens.
+ * out = softmax(scale * q.k) . v per head, kv head h / (n_head/n_head_kv);
+ * scale 0 takes 1/sqrt(head_dim).  q and out: head h of row r at r*stride +
+ * h*head_dim.  head_dim 64, 128 or 256, any group size.  ctx_len is cut at
+ * max_ctx (and max_pages*page); a row with no tokens gives zeros; tokens on a page
+ * outside [0, n_pages) are left out.  Scores, sums and outputs are held in fp32; for
+ * F32 queries the products carry 22 bits of each factor, for F16 and BF16
+ * queries the queries' own. */
+MV_API int mv_paged_attn_q4(int type, const void* q_dev, uint64_t q_row_stride, uint64_t n_seq, uint64_t n_head,
+                            uint64_t n_head_kv, uint64_t head_dim, const void* k_pages_dev, const void* v_pages_dev,
+                            const void* k_scales_dev, const void* v_scales_dev, const int32_t* block_table_dev,
+                            uint64_t max_pages, uint64_t page, uint64_t n_pages, const int32_t* ctx_len_dev,
+                            uint64_t max_ctx, float scale, void* out_dev, uint64_t out_row_stride, void* stream);
+/* The same for chunks of query rows: sequence s owns rows q_start[s] ..
+ * q_start[s+1] of the n_q rows (device array of n_seq + 1, ascending from 0 to
+ * n_q), at most max_q of them; row r attends to its first ctx_len[r] tokens
+ * (causal: start + i + 1). */
+MV_API int mv_paged_attn_q4_prefill(int type, const void* q_dev, uint64_t q_row_stride, uint64_t n_q, uint64_t n_head,
+                                    uint64_t n_head_kv, uint64_t head_dim, const void* k_pages_dev,
+                                    const void* v_pages_dev, const void* k_scales_dev, const void* v_scales_dev,
+                                    const int32_t* block_table_dev, uint64_t n_seq, uint64_t max_pages, uint64_t page,
+                                    uint64_t n_pages, const int32_t* q_start_dev, uint64_t max_q,
+                                    const int32_t* ctx_len_dev, uint64_t max_ctx, float scale, void* out_dev,
+                                    uint64_t out_row_stride, void* stream);
 
 /* ---------------------------------- host-pointer calls (reference contract) */
 

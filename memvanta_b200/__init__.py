@@ -21,14 +21,16 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import (F32, F16, Q4_0, Q8_0, Q6_K, ACT_F32, ACT_Q8, KV_F32, KV_F16, KV_Q8, KV_Q8_0,  # noqa: F401
-                   MV_ERR_TIMEOUT, MemVantaError, check, load)
+from ._lib import (F32, F16, BF16, Q4_0, Q8_0, Q6_K, ACT_F32, ACT_Q8, KV_F32, KV_F16, KV_Q8, KV_Q8_0,  # noqa: F401
+                   KV_Q4_0, MV_ERR_TIMEOUT, ROPE_HALF, ROPE_INTERLEAVED, ROPE_SCALE_BANDS, ROPE_SCALE_LINEAR,
+                   ROPE_SCALE_NONE, ROPE_SCALE_YARN, MemVantaError, check, load)
 
 __all__ = [
     "init", "Weight", "tensor_matvec", "tensor_matmul_batch", "tensor_matmul_batch_v06", "tensor_read_row_f32",
     "gemv", "gemm", "quantize_q8", "q4_0_block_dots", "read_rows", "rmsnorm", "rope", "silu_mul", "add_inplace",
-    "fp32_to_fp16", "kv_row_bytes", "kv_row_scales", "kv_append", "paged_attn_decode", "paged_attn_prefill", "LlamaModel",
-    "SequenceSet",
+    "fp32_to_fp16", "kv_row_bytes", "kv_row_scales", "kv_append", "paged_attn_decode", "paged_attn_prefill",
+    "rope_table", "rope_apply", "kv_pools", "rope_kv_append", "kv_read", "paged_attn_q4", "paged_attn_q4_prefill",
+    "LlamaModel", "SequenceSet",
     "MemVantaError",
 ]
 
@@ -320,6 +322,240 @@ def paged_attn_prefill(kv_type, q, n_head, n_head_kv, head_dim, k_pages, v_pages
     check(load().mv_paged_attn_prefill(kv_type, _t_ptr(q), n_q, n_head, n_head_kv, head_dim, _t_ptr(k_pages),
                                        _t_ptr(v_pages), _t_ptr(k_scales), _t_ptr(v_scales), _t_ptr(block_table),
                                        max_pages, page, _t_ptr(ctx_len), max_ctx, _t_ptr(out), _stream(stream)))
+    return out
+
+
+# ---- rotary positions and the 4-bit cache.  Activations are [rows, heads,
+# head_dim] CUDA tensors (float32, float16 or bfloat16) whose heads may lie
+# anywhere as long as a head's dimensions are next to one another.
+
+_ACT = {}
+
+
+def _act_type(t) -> int:
+    if not _ACT:
+        import torch
+        _ACT.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    try:
+        return _ACT[t.dtype]
+    except KeyError:
+        raise MemVantaError(_lib.MV_ERR_UNSUPPORTED, f"activations must be float32, float16 or bfloat16, not {t.dtype}")
+
+
+def _bad(msg: str):
+    raise MemVantaError(_lib.MV_ERR_INVALID, msg)
+
+
+def _heads(name: str, t, rows: int | None = None, hd: int | None = None):
+    """Row and head stride of an activation tensor, checked."""
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        _bad(f"{name} must be [rows, heads, head_dim] with a head's dimensions next to one another")
+    if rows is not None and t.shape[0] != rows or hd is not None and t.shape[2] != hd:
+        _bad(f"{name} is {tuple(t.shape)}: rows or head_dim differ from the other tensors'")
+    return t.stride(0), t.stride(1)
+
+
+def _i32(name: str, t, n: int | None = None):
+    if t is None:
+        return None
+    if str(t.dtype) != "torch.int32" or not t.is_contiguous() or (n is not None and t.numel() != n):
+        _bad(f"{name} must be a contiguous int32 tensor" + ("" if n is None else f" of {n} elements"))
+    return t.data_ptr()
+
+
+def _rope_tables(cos_t, sin_t, rot_dim, head_dim):
+    """(rot_dim, rows of the tables); without tables nothing is rotated."""
+    if cos_t is None and sin_t is None and not rot_dim:
+        return 0, 0
+    if cos_t is None or sin_t is None or cos_t.shape != sin_t.shape or cos_t.dim() != 2 or \
+            not (cos_t.is_contiguous() and sin_t.is_contiguous()) or str(cos_t.dtype) != "torch.float32" or \
+            str(sin_t.dtype) != "torch.float32":
+        _bad("cos and sin must be contiguous float32 tables [n_pos, rot_dim / 2]")
+    if rot_dim is None:
+        rot_dim = 2 * cos_t.shape[1]
+    if 2 * cos_t.shape[1] != rot_dim or rot_dim > head_dim:
+        _bad(f"the tables hold {cos_t.shape[1]} angles per position: rot_dim {rot_dim}, head_dim {head_dim}")
+    return rot_dim, cos_t.shape[0]
+
+
+def rope_table(rot_dim: int, n_pos: int, theta: float = 10000.0, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0,
+               orig_ctx: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0,
+               freq_factors=None, device=None, stream=None):
+    """cos and sin tables [n_pos, rot_dim / 2] (mv_rope_table)."""
+    import torch
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    cos_t = torch.empty((n_pos, rot_dim // 2), dtype=torch.float32, device=dev)
+    sin_t = torch.empty_like(cos_t)
+    if freq_factors is not None and (freq_factors.dtype != torch.float32 or not freq_factors.is_contiguous()
+                                     or freq_factors.numel() != rot_dim // 2):
+        _bad("freq_factors must be a contiguous float32 tensor of rot_dim / 2 elements")
+    check(load().mv_rope_table(rot_dim, n_pos, theta, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor,
+                               _t_ptr(freq_factors), _t_ptr(cos_t), _t_ptr(sin_t), _stream(stream)))
+    return cos_t, sin_t
+
+
+def rope_apply(x, cos_t, sin_t, pos, layout: int = ROPE_HALF, rot_dim: int | None = None, out=None, stream=None):
+    """x [rows, heads, head_dim] with the first rot_dim (default: the tables'
+    width) dimensions of each head rotated by its row's position; out may be x."""
+    rows, n_head, hd = x.shape
+    if out is None:
+        import torch
+        out = torch.empty((rows, n_head, hd), dtype=x.dtype, device=x.device)
+    elif out.dtype != x.dtype or out.shape != x.shape:
+        _bad("out must have x's shape and type")
+    xs, os_ = _heads("x", x), _heads("out", out)
+    rot_dim, n_pos = _rope_tables(cos_t, sin_t, rot_dim, hd)
+    check(load().mv_rope_apply(_act_type(x), x.data_ptr(), xs[0], xs[1], out.data_ptr(), os_[0], os_[1], rows, n_head,
+                               hd, rot_dim, layout, _t_ptr(cos_t), _t_ptr(sin_t), n_pos, _i32("pos", pos, rows),
+                               _stream(stream)))
+    return out
+
+
+def kv_pools(kv_type: int, n_pages: int, page: int, n_head_kv: int, head_dim: int, device=None):
+    """Empty (zeroed) pools (k_pages, v_pages, k_scales, v_scales) of a paged
+    cache; the scales are None for the types that have none."""
+    import torch
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    kv_dim, slots = n_head_kv * head_dim, n_pages * page
+    shape, dtype = {KV_F32: ((n_pages, page, n_head_kv, head_dim), torch.float32),
+                    KV_F16: ((n_pages, page, n_head_kv, head_dim), torch.float16),
+                    KV_Q8: ((n_pages, page, n_head_kv, head_dim), torch.int8),
+                    KV_Q8_0: ((n_pages, page, n_head_kv, head_dim), torch.int8),
+                    KV_Q4_0: ((n_pages, n_head_kv, page, head_dim // 2), torch.uint8)}[kv_type]
+    pages = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(2)]
+    if kv_type == KV_Q4_0:
+        scales = [torch.zeros((n_pages, n_head_kv, page, head_dim // 32), dtype=torch.bfloat16, device=dev)
+                  for _ in range(2)]
+    elif kv_type in (KV_Q8, KV_Q8_0):
+        scales = [torch.zeros((slots, kv_row_scales(kv_type, kv_dim)), dtype=torch.float32, device=dev)
+                  for _ in range(2)]
+    else:
+        scales = [None, None]
+    return pages[0], pages[1], scales[0], scales[1]
+
+
+_KV_ELEMENT = {KV_F32: 4, KV_F16: 2, KV_Q8: 1, KV_Q8_0: 1}
+
+
+def _pool_pages(kv_type: int, pages, scales, page: int, n_head_kv: int, head_dim: int) -> int:
+    """Pages that a pool's tensor holds, its scales checked against it."""
+    if kv_type != KV_Q4_0 and kv_type not in _KV_ELEMENT:
+        raise MemVantaError(_lib.MV_ERR_UNSUPPORTED, "unknown KV cache type")
+    kv_dim = n_head_kv * head_dim
+    if not pages.is_contiguous() or (scales is not None and not scales.is_contiguous()):
+        _bad("cache pages and scales must be contiguous")
+    per = page * kv_dim // 2 if kv_type == KV_Q4_0 else page * kv_dim * _KV_ELEMENT[kv_type]
+    n = pages.numel() * pages.element_size() // per if per else 0
+    if kv_type >= KV_Q8 and scales is not None:
+        need = n * page * (1 if kv_type == KV_Q8 else kv_dim // 32)
+        if scales.numel() < need or scales.element_size() != (2 if kv_type == KV_Q4_0 else 4):
+            _bad("the scale array does not fit the pages")
+    return n
+
+
+def _table(block_table):
+    if block_table.dim() != 2:
+        _bad("block_table must be [n_seq, max_pages]")
+    return _i32("block_table", block_table), block_table.shape[0], block_table.shape[1]
+
+
+def rope_kv_append(kv_type: int, q, k, v, cos_t, sin_t, pos, block_table, page: int, k_pages, v_pages, k_scales=None,
+                   v_scales=None, seq=None, layout: int = ROPE_HALF, rot_dim: int | None = None, q_out=None,
+                   stream=None):
+    """Rotates q (may be None) into q_out and k into the paged cache, and stores
+    v (mv_rope_kv_append); returns q_out.  Without tables nothing is rotated."""
+    rows, n_head_kv, hd = k.shape
+    ks, vs = _heads("k", k), _heads("v", v, rows, hd)
+    if v.shape[1] != n_head_kv or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        _bad("q, k and v must have one type, k and v the same heads")
+    n_head, qs, os_ = 0, (0, 0), (0, 0)
+    if q is not None:
+        qs, n_head = _heads("q", q, rows, hd), q.shape[1]
+        if q_out is None:
+            import torch
+            q_out = torch.empty((rows, n_head, hd), dtype=q.dtype, device=q.device)
+        elif q_out.dtype != q.dtype or q_out.shape != q.shape:
+            _bad("q_out must have q's shape and type")
+        os_ = _heads("q_out", q_out)
+    rot_dim, n_pos = _rope_tables(cos_t, sin_t, rot_dim, hd)
+    n_pages = min(_pool_pages(kv_type, k_pages, k_scales, page, n_head_kv, hd),
+                  _pool_pages(kv_type, v_pages, v_scales, page, n_head_kv, hd))
+    table, n_seq, max_pages = _table(block_table)
+    check(load().mv_rope_kv_append(
+        kv_type, _act_type(k), None if q is None else q.data_ptr(), qs[0], qs[1],
+        None if q is None else q_out.data_ptr(), os_[0], os_[1], n_head, k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+        vs[0], vs[1], n_head_kv, rows, hd, rot_dim, layout, _t_ptr(cos_t), _t_ptr(sin_t), n_pos,
+        _i32("seq", seq, rows), _i32("pos", pos, rows), table, n_seq, max_pages, page, n_pages, k_pages.data_ptr(),
+        v_pages.data_ptr(), _t_ptr(k_scales), _t_ptr(v_scales), _stream(stream)))
+    return q_out
+
+
+def kv_read(kv_type: int, pages, scales, pos, block_table, page: int, n_head_kv: int, head_dim: int, seq=None,
+            dtype=None, out=None, stream=None):
+    """Cached rows of one pool as the values they stand for: [rows, n_head_kv,
+    head_dim] of dtype (default float32) (mv_kv_read)."""
+    import torch
+    rows = pos.numel()
+    if out is None:
+        out = torch.empty((rows, n_head_kv, head_dim), dtype=dtype or torch.float32, device=pages.device)
+    elif tuple(out.shape) != (rows, n_head_kv, head_dim) or not out.is_contiguous():
+        _bad("out must be a contiguous [rows, n_head_kv, head_dim] tensor")
+    n_pages = _pool_pages(kv_type, pages, scales, page, n_head_kv, head_dim)
+    table, n_seq, max_pages = _table(block_table)
+    check(load().mv_kv_read(kv_type, pages.data_ptr(), _t_ptr(scales), n_head_kv, head_dim, rows,
+                            _i32("seq", seq, rows), _i32("pos", pos, rows), table, n_seq, max_pages, page, n_pages,
+                            _act_type(out), out.data_ptr(), _stream(stream)))
+    return out
+
+
+def _q4_args(q, k_pages, v_pages, k_scales, v_scales, out):
+    """Checked (type, strides, sizes) of a 4-bit attention call; pools as kv_pools shapes them."""
+    rows, n_head, hd = q.shape
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] * 2 != hd:
+        _bad("pools must be [n_pages, n_head_kv, page, head_dim / 2], the same for k and v")
+    n_pages, n_head_kv, page, _ = k_pages.shape
+    for p, s in ((k_pages, k_scales), (v_pages, v_scales)):
+        if p.element_size() != 1 or s is None or _pool_pages(KV_Q4_0, p, s, page, n_head_kv, hd) != n_pages:
+            _bad("pools must hold bytes, with their scales")
+    if out is None:
+        import torch
+        out = torch.empty((rows, n_head, hd), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        _bad("out must have q's shape and type")
+    qs, os_ = _heads("q", q), _heads("out", out)
+    if n_head > 1 and (qs[1] != hd or os_[1] != hd):
+        _bad("the heads of a query row must be next to one another")
+    # a tensor of one row may carry any stride
+    qr, orow = (n_head * hd, n_head * hd) if rows == 1 else (qs[0], os_[0])
+    return out, _act_type(q), qr, orow, n_head, n_head_kv, hd, page, n_pages
+
+
+def paged_attn_q4(q, k_pages, v_pages, k_scales, v_scales, block_table, ctx_len, max_ctx: int, scale: float = 0.0,
+                  out=None, stream=None):
+    """Attention over a 4-bit cache, one query row per sequence: q [n_seq,
+    heads, head_dim], row i sees its first ctx_len[i] tokens (mv_paged_attn_q4)."""
+    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out)
+    table, n_seq, max_pages = _table(block_table)
+    if n_seq != q.shape[0]:
+        _bad(f"the block table has {n_seq} sequences, q {q.shape[0]} rows")
+    check(load().mv_paged_attn_q4(ty, q.data_ptr(), qr, n_seq, n_head, n_head_kv, hd, k_pages.data_ptr(),
+                                  v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), table, max_pages, page,
+                                  n_pages, _i32("ctx_len", ctx_len, n_seq), max_ctx, scale, out.data_ptr(), orow,
+                                  _stream(stream)))
+    return out
+
+
+def paged_attn_q4_prefill(q, k_pages, v_pages, k_scales, v_scales, block_table, q_start, max_q: int, ctx_len,
+                          max_ctx: int, scale: float = 0.0, out=None, stream=None):
+    """The same for chunks of query rows: sequence s owns rows q_start[s] ..
+    q_start[s + 1] of q, row r sees ctx_len[r] tokens (mv_paged_attn_q4_prefill)."""
+    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out)
+    table, n_seq, max_pages = _table(block_table)
+    check(load().mv_paged_attn_q4_prefill(ty, q.data_ptr(), qr, q.shape[0], n_head, n_head_kv, hd, k_pages.data_ptr(),
+                                          v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), table, n_seq,
+                                          max_pages, page, n_pages, _i32("q_start", q_start, n_seq + 1), max_q,
+                                          _i32("ctx_len", ctx_len, q.shape[0]), max_ctx, scale, out.data_ptr(), orow,
+                                          _stream(stream)))
     return out
 
 

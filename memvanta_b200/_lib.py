@@ -16,14 +16,17 @@ LIB_PATH = os.path.join(HERE, "libmemvanta_b200.so")
 MV_OK, MV_ERR_INVALID, MV_ERR_UNSUPPORTED, MV_ERR_CUDA, MV_ERR_OOM, MV_ERR_IO, MV_ERR_TIMEOUT, MV_ERR_NOT_BUILT = range(8)
 ERR_NAMES = {1: "MV_ERR_INVALID", 2: "MV_ERR_UNSUPPORTED", 3: "MV_ERR_CUDA", 4: "MV_ERR_OOM", 5: "MV_ERR_IO",
              6: "MV_ERR_TIMEOUT", 7: "MV_ERR_NOT_BUILT"}
-F32, F16, Q4_0, Q8_0, Q6_K = 0, 1, 2, 8, 14
+F32, F16, Q4_0, Q8_0, Q6_K, BF16 = 0, 1, 2, 8, 14, 30
 ACT_F32, ACT_Q8 = 0, 1
-KV_F32, KV_F16, KV_Q8, KV_Q8_0 = 0, 1, 2, 3
+KV_F32, KV_F16, KV_Q8, KV_Q8_0, KV_Q4_0 = 0, 1, 2, 3, 4
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN, ROPE_SCALE_BANDS = 0, 1, 2, 3
 
 _p = C.c_void_p
 _u64 = C.c_uint64
 _i = C.c_int
 _f = C.c_float
+_d = C.c_double
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -59,6 +62,16 @@ SIGNATURES = {
                                         _p, _p]),
     "mv_paged_attn_prefill": (_i, [_i, _p, _u64, _u64, _u64, _u64, _p, _p, _p, _p, _p, _u64, _u64, _p, _u64, _p,
                                    _p]),
+    "mv_rope_table": (_i, [_u64, _u64, _d, _i, _d, _d, _d, _d, _d, _p, _p, _p, _p]),
+    "mv_rope_apply": (_i, [_i, _p, _u64, _u64, _p, _u64, _u64, _u64, _u64, _u64, _u64, _i, _p, _p, _u64, _p, _p]),
+    "mv_rope_kv_append": (_i, [_i, _i, _p, _u64, _u64, _p, _u64, _u64, _u64, _p, _u64, _u64, _p, _u64, _u64, _u64,
+                               _u64, _u64, _u64, _i, _p, _p, _u64, _p, _p, _p, _u64, _u64, _u64, _u64, _p, _p, _p,
+                               _p, _p]),
+    "mv_kv_read": (_i, [_i, _p, _p, _u64, _u64, _u64, _p, _p, _p, _u64, _u64, _u64, _u64, _i, _p, _p]),
+    "mv_paged_attn_q4": (_i, [_i, _p, _u64, _u64, _u64, _u64, _u64, _p, _p, _p, _p, _p, _u64, _u64, _u64, _p, _u64,
+                              _f, _p, _u64, _p]),
+    "mv_paged_attn_q4_prefill": (_i, [_i, _p, _u64, _u64, _u64, _u64, _u64, _p, _p, _p, _p, _p, _u64, _u64, _u64,
+                                      _u64, _p, _u64, _p, _u64, _f, _p, _u64, _p]),
     "mv_tensor_matvec_host": (_i, [_p, _p, _p]),
     "mv_tensor_matmul_batch_host": (_i, [_p, _p, _p, _u64, _i]),
     "mv_tensor_read_row_host": (_i, [_p, _u64, _p]),

@@ -17,9 +17,11 @@
 namespace mvb {
 
 uint64_t kv_row_bytes(int kv_type, uint64_t kv_dim) {
-    return kv_type == 0 ? kv_dim * 4 : kv_type == 1 ? kv_dim * 2 : kv_dim;
+    return kv_type == 0 ? kv_dim * 4 : kv_type == 1 ? kv_dim * 2 : kv_type == 4 ? kv_dim / 2 : kv_dim;
 }
-uint64_t kv_row_scales(int kv_type, uint64_t kv_dim) { return kv_type == 2 ? 1 : kv_type == 3 ? kv_dim / 32 : 0; }
+uint64_t kv_row_scales(int kv_type, uint64_t kv_dim) {
+    return kv_type == 2 ? 1 : kv_type == 3 || kv_type == 4 ? kv_dim / 32 : 0;
+}
 
 // ---------------------------------------------------------------- append
 // One CTA per (token row, K|V).  F16 uses the reference's fp32_to_fp16; Q8

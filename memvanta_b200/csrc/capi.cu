@@ -5,6 +5,8 @@
 // codes; CUDA failures come back as MV_ERR_CUDA with the runtime's message.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -467,6 +469,196 @@ MV_API int mv_paged_attn_prefill(int kv_type, const float* q, uint64_t n_q, uint
                     block_table, max_pages, page, ctx_len, max_ctx ? max_ctx : 1, out};
     a.one_seq = 1;
     CK(mvb::paged_attn_prefill(a, as_stream(stream)));
+    return MV_OK;
+}
+
+// ------------------------------- rotary positions and the 4-bit cache
+namespace {
+
+int check_act_type(int type) {
+    if (type != MV_TYPE_F32 && type != MV_TYPE_F16 && type != MV_TYPE_BF16)
+        return fail(MV_ERR_UNSUPPORTED, "activations must be F32, F16 or BF16");
+    return MV_OK;
+}
+int check_rope(uint64_t head_dim, uint64_t rot_dim, int layout, const float* cos_t, const float* sin_t) {
+    if (rot_dim % 2 || rot_dim > head_dim) return fail(MV_ERR_INVALID, "rot_dim must be even and at most head_dim");
+    if (layout != MV_ROPE_HALF && layout != MV_ROPE_INTERLEAVED) return fail(MV_ERR_INVALID, "unknown rotary layout");
+    if (rot_dim && (!cos_t || !sin_t)) return fail(MV_ERR_INVALID, "null cos or sin table");
+    return MV_OK;
+}
+int check_rows(uint64_t rows, uint64_t n_head, uint64_t head_dim) {
+    // kernels index one row's items and the grid with 32-bit integers
+    if (rows > 0x7fffffffull || n_head > 65535 || head_dim > 65536 || n_head * head_dim > (1ull << 24))
+        return fail(MV_ERR_INVALID, "too many rows or heads");
+    return MV_OK;
+}
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+int check_cache(int kv_type, uint64_t n_head_kv, uint64_t head_dim, const void* pages, const void* scales) {
+    if (kv_type < 0 || kv_type > 4) return fail(MV_ERR_UNSUPPORTED, "unknown KV cache type");
+    if (!pages) return fail(MV_ERR_INVALID, "null pages");
+    if (kv_type >= 2 && !scales) return fail(MV_ERR_INVALID, "Q8 and Q4 caches need scale arrays");
+    if (head_dim % (kv_type >= 3 ? 32 : 8))
+        return fail(MV_ERR_INVALID, kv_type >= 3 ? "Q8_0 and Q4_0 caches need head_dim % 32 == 0"
+                                                 : "the cache calls need head_dim % 8 == 0");
+    if (!n_head_kv || !head_dim) return fail(MV_ERR_INVALID, "n_head_kv and head_dim must be > 0");
+    if (misaligned(pages) || (kv_type == 4 && misaligned(scales)))
+        return fail(MV_ERR_INVALID, "cache pages and 4-bit scales must be 16-byte aligned");
+    return MV_OK;
+}
+int check_table(const int32_t* table, const int32_t* pos, uint64_t n_seq, uint64_t max_pages, uint64_t page,
+                uint64_t n_pages) {
+    if (!table || !pos) return fail(MV_ERR_INVALID, "null block table or per-row array");
+    if (!page || page > 0x7fffffffull) return fail(MV_ERR_INVALID, "page must be > 0");
+    if (!n_seq || !max_pages) return fail(MV_ERR_INVALID, "the block table needs n_seq > 0 and max_pages > 0");
+    if (n_seq > 0x7fffffffull || n_pages > 0x7fffffffull || max_pages > 0x7fffffffull / page)
+        return fail(MV_ERR_INVALID, "max_pages * page, n_pages and n_seq must stay below 2^31");
+    return MV_OK;
+}
+// Attention calls: everything but the row layout.
+int check_attn_q4(int type, const void* q, uint64_t q_stride, uint64_t n_head, uint64_t n_head_kv, uint64_t hd,
+                  const void* kp, const void* vp, const void* ks, const void* vs, float scale, const void* out,
+                  uint64_t out_stride) {
+    if (int rc = check_act_type(type)) return rc;
+    if (!n_head || !n_head_kv || n_head % n_head_kv)
+        return fail(MV_ERR_INVALID, "n_head must be a multiple of n_head_kv");
+    if (hd != 64 && hd != 128 && hd != 256) return fail(MV_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+    if (!q || !out) return fail(MV_ERR_INVALID, "null q or out");
+    const uint64_t e = type == MV_TYPE_F32 ? 4 : 2;
+    if (misaligned(q) || misaligned(out) || q_stride * e % 16 || out_stride * e % 16)
+        return fail(MV_ERR_INVALID, "q and out rows must start 16-byte aligned");
+    if (q_stride < n_head * hd || out_stride < n_head * hd)
+        return fail(MV_ERR_INVALID, "row strides must hold n_head * head_dim elements");
+    if (!(scale >= 0.0f) || scale > 3.0e38f) return fail(MV_ERR_INVALID, "scale must be finite and >= 0");
+    if (int rc = check_cache(MV_KV_Q4_0, n_head_kv, hd, kp, ks)) return rc;
+    return check_cache(MV_KV_Q4_0, n_head_kv, hd, vp, vs);
+}
+
+}  // namespace
+
+MV_API int mv_rope_table(uint64_t rot_dim, uint64_t n_pos, double theta, int scaling, double factor, double orig_ctx,
+                         double beta_fast, double beta_slow, double attn_factor, const float* freq_factors,
+                         float* cos_t, float* sin_t, void* stream) {
+    if (!rot_dim || rot_dim % 2 || rot_dim > 65536) return fail(MV_ERR_INVALID, "rot_dim must be even and > 0");
+    if (n_pos > 0x7fffffffull) return fail(MV_ERR_INVALID, "too many positions");
+    if (!(theta > 1.0) || theta > 1e300) return fail(MV_ERR_INVALID, "theta must be above 1");
+    if (scaling < MV_ROPE_SCALE_NONE || scaling > MV_ROPE_SCALE_BANDS)
+        return fail(MV_ERR_INVALID, "unknown rotary scaling");
+    if (scaling && (!(factor > 0.0) || factor > 1e300)) return fail(MV_ERR_INVALID, "the scaling factor must be > 0");
+    if (scaling >= MV_ROPE_SCALE_YARN && (!(orig_ctx > 0.0) || !(beta_slow > 0.0) || !(beta_fast > beta_slow) ||
+                                          !(beta_fast < 1e300) || !(orig_ctx < 1e300) || !(attn_factor >= 0.0)))
+        return fail(MV_ERR_INVALID, "this scaling needs orig_ctx > 0, beta_fast > beta_slow > 0 and attn_factor >= 0");
+    if (n_pos && (!cos_t || !sin_t)) return fail(MV_ERR_INVALID, "null cos or sin table");
+    mvb::RopeScaling r{scaling, theta, factor, orig_ctx, beta_fast, beta_slow, attn_factor};
+    CK(mvb::rope_table(r, rot_dim, n_pos, freq_factors, cos_t, sin_t, as_stream(stream)));
+    return MV_OK;
+}
+
+MV_API int mv_rope_apply(int type, const void* x, uint64_t x_row_stride, uint64_t x_head_stride, void* out,
+                         uint64_t out_row_stride, uint64_t out_head_stride, uint64_t rows, uint64_t n_head,
+                         uint64_t head_dim, uint64_t rot_dim, int layout, const float* cos_t, const float* sin_t,
+                         uint64_t n_pos, const int32_t* pos, void* stream) {
+    if (int rc = check_act_type(type)) return rc;
+    if (int rc = check_rope(head_dim, rot_dim, layout, cos_t, sin_t)) return rc;
+    if (int rc = check_rows(rows, n_head, head_dim)) return rc;
+    if (!rot_dim || head_dim % 2) return fail(MV_ERR_INVALID, "rot_dim must be > 0 and head_dim even");
+    if (rows == 0 || n_head == 0) return MV_OK;
+    if (!x || !out || !pos) return fail(MV_ERR_INVALID, "null x, out or pos");
+    if (x == out && (x_row_stride != out_row_stride || x_head_stride != out_head_stride))
+        return fail(MV_ERR_INVALID, "in place needs equal strides");
+    mvb::RopeApplyArgs a{x, x_row_stride, x_head_stride, out, out_row_stride, out_head_stride, n_head, head_dim,
+                         rot_dim, layout, cos_t, sin_t, n_pos, pos};
+    CK(mvb::rope_apply(type, a, rows, as_stream(stream)));
+    return MV_OK;
+}
+
+MV_API int mv_rope_kv_append(int kv_type, int type, const void* q, uint64_t q_row_stride, uint64_t q_head_stride,
+                             void* q_out, uint64_t q_out_row_stride, uint64_t q_out_head_stride, uint64_t n_head,
+                             const void* k, uint64_t k_row_stride, uint64_t k_head_stride, const void* v,
+                             uint64_t v_row_stride, uint64_t v_head_stride, uint64_t n_head_kv, uint64_t rows,
+                             uint64_t head_dim, uint64_t rot_dim, int layout, const float* cos_t, const float* sin_t,
+                             uint64_t n_pos, const int32_t* seq, const int32_t* pos, const int32_t* block_table,
+                             uint64_t n_seq, uint64_t max_pages, uint64_t page, uint64_t n_pages, void* k_pages,
+                             void* v_pages, void* k_scales, void* v_scales, void* stream) {
+    if (int rc = check_act_type(type)) return rc;
+    if (int rc = check_rope(head_dim, rot_dim, layout, cos_t, sin_t)) return rc;
+    if (int rc = check_rows(rows, n_head, head_dim)) return rc;
+    if (int rc = check_rows(rows, n_head_kv, head_dim)) return rc;
+    if (int rc = check_cache(kv_type, n_head_kv, head_dim, k_pages, k_scales)) return rc;
+    if (int rc = check_cache(kv_type, n_head_kv, head_dim, v_pages, v_scales)) return rc;
+    if (rows == 0) return MV_OK;
+    if (int rc = check_table(block_table, pos, n_seq, max_pages, page, n_pages)) return rc;
+    if (!k || !v || (n_head && (!q || !q_out))) return fail(MV_ERR_INVALID, "null q, q_out, k or v");
+    if (n_head && q == q_out && (q_row_stride != q_out_row_stride || q_head_stride != q_out_head_stride))
+        return fail(MV_ERR_INVALID, "in place needs equal strides");
+    mvb::RopeAppendArgs a{};
+    a.kv_type = kv_type;
+    a.q = {q, q_row_stride, q_head_stride, q_out, q_out_row_stride, q_out_head_stride, n_head, head_dim,
+           rot_dim, layout, cos_t, sin_t, n_pos, pos};
+    a.k = k, a.k_stride = k_row_stride, a.k_head_stride = k_head_stride;
+    a.v = v, a.v_stride = v_row_stride, a.v_head_stride = v_head_stride;
+    a.n_head_kv = n_head_kv, a.hd = head_dim, a.rot = rot_dim, a.layout = layout;
+    a.cos_t = cos_t, a.sin_t = sin_t, a.n_pos = n_pos, a.n_rows = rows;
+    a.rows = {seq, pos, block_table, n_seq, max_pages, page, n_pages};
+    a.k_pages = k_pages, a.v_pages = v_pages, a.k_scales = k_scales, a.v_scales = v_scales;
+    CK(mvb::rope_kv_append(type, a, as_stream(stream)));
+    return MV_OK;
+}
+
+MV_API int mv_kv_read(int kv_type, const void* pages, const void* scales, uint64_t n_head_kv, uint64_t head_dim,
+                      uint64_t rows, const int32_t* seq, const int32_t* pos, const int32_t* block_table,
+                      uint64_t n_seq, uint64_t max_pages, uint64_t page, uint64_t n_pages, int out_type, void* out,
+                      void* stream) {
+    if (int rc = check_act_type(out_type)) return rc;
+    if (int rc = check_rows(rows, n_head_kv, head_dim)) return rc;
+    if (int rc = check_cache(kv_type, n_head_kv, head_dim, pages, scales)) return rc;
+    if (rows == 0) return MV_OK;
+    if (int rc = check_table(block_table, pos, n_seq, max_pages, page, n_pages)) return rc;
+    if (!out || misaligned(out)) return fail(MV_ERR_INVALID, "out must be a 16-byte aligned pointer");
+    mvb::KvReadArgs a{kv_type, pages, scales, n_head_kv, head_dim,
+                      {seq, pos, block_table, n_seq, max_pages, page, n_pages}, out};
+    CK(mvb::kv_read(out_type, a, rows, as_stream(stream)));
+    return MV_OK;
+}
+
+MV_API int mv_paged_attn_q4(int type, const void* q, uint64_t q_row_stride, uint64_t n_seq, uint64_t n_head,
+                            uint64_t n_head_kv, uint64_t hd, const void* k_pages, const void* v_pages,
+                            const void* k_scales, const void* v_scales, const int32_t* block_table,
+                            uint64_t max_pages, uint64_t page, uint64_t n_pages, const int32_t* ctx_len,
+                            uint64_t max_ctx, float scale, void* out, uint64_t out_row_stride, void* stream) {
+    if (n_seq == 0) return MV_OK;
+    if (int rc = check_attn_q4(type, q, q_row_stride, n_head, n_head_kv, hd, k_pages, v_pages, k_scales, v_scales,
+                               scale, out, out_row_stride))
+        return rc;
+    if (int rc = check_rows(n_seq, n_head, hd)) return rc;
+    if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    mvb::AttnQ4Args a{q, q_row_stride, n_seq, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
+                      static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
+                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, nullptr, 1,
+                      ctx_len, std::min(max_ctx, max_pages * page),
+                      scale > 0.0f ? scale : 1.0f / std::sqrt((float)hd), out, out_row_stride};
+    CK(mvb::attn_q4(type, a, as_stream(stream)));
+    return MV_OK;
+}
+
+MV_API int mv_paged_attn_q4_prefill(int type, const void* q, uint64_t q_row_stride, uint64_t n_q, uint64_t n_head,
+                                    uint64_t n_head_kv, uint64_t hd, const void* k_pages, const void* v_pages,
+                                    const void* k_scales, const void* v_scales, const int32_t* block_table,
+                                    uint64_t n_seq, uint64_t max_pages, uint64_t page, uint64_t n_pages,
+                                    const int32_t* q_start, uint64_t max_q, const int32_t* ctx_len, uint64_t max_ctx,
+                                    float scale, void* out, uint64_t out_row_stride, void* stream) {
+    if (n_q == 0) return MV_OK;
+    if (int rc = check_attn_q4(type, q, q_row_stride, n_head, n_head_kv, hd, k_pages, v_pages, k_scales, v_scales,
+                               scale, out, out_row_stride))
+        return rc;
+    if (int rc = check_rows(n_q, n_head, hd)) return rc;
+    if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    if (!q_start || !max_q || max_q > n_q) return fail(MV_ERR_INVALID, "prefill needs q_start and max_q in 1..n_q");
+    mvb::AttnQ4Args a{q, q_row_stride, n_q, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
+                      static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
+                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, q_start,
+                      max_q, ctx_len, std::min(max_ctx, max_pages * page),
+                      scale > 0.0f ? scale : 1.0f / std::sqrt((float)hd), out, out_row_stride};
+    CK(mvb::attn_q4(type, a, as_stream(stream)));
     return MV_OK;
 }
 

@@ -162,6 +162,85 @@ struct AttnArgs {
     uint64_t xq_ldb = 0;
     bool xq_f16 = false;  // xq holds fp16 values of the Q8 integers (the fp16 GEMM's input)
 };
+// ---- rope_kv.cu : rotary positions, and the append of rotated keys and of
+// values to the paged cache.  Strides are in elements; `type` is a GGML type id
+// (0 F32, 1 F16, 30 BF16); layout 0 pairs (i, i + rot/2), 1 pairs (2i, 2i+1).
+struct RopeScaling {
+    int kind;  // 0 none, 1 linear, 2 YaRN, 3 wavelength bands
+    double theta, factor, orig_ctx, beta_fast, beta_slow, attn_factor;
+};
+cudaError_t rope_table(const RopeScaling& r, uint64_t rot, uint64_t n_pos, const float* factors, float* cos_t,
+                       float* sin_t, cudaStream_t s);
+struct RopeApplyArgs {  // head h of row r at x + r * x_stride + h * x_head_stride
+    const void* x;
+    uint64_t x_stride, x_head_stride;
+    void* out;
+    uint64_t out_stride, out_head_stride;
+    uint64_t n_head, hd, rot;
+    int layout;
+    const float* cos_t;  // [n_pos][rot / 2]
+    const float* sin_t;
+    uint64_t n_pos;
+    const int32_t* pos;  // per row
+};
+cudaError_t rope_apply(int type, const RopeApplyArgs& a, uint64_t rows, cudaStream_t s);
+struct KvRows {  // cache rows by sequence and position
+    const int32_t* seq;  // per row; nullptr: all sequence 0
+    const int32_t* pos;
+    const int32_t* block_table;  // [n_seq][max_pages]
+    uint64_t n_seq, max_pages, page, n_pages;
+};
+struct RopeAppendArgs {
+    int kv_type;
+    RopeApplyArgs q;  // n_head 0: no queries
+    const void* k;
+    uint64_t k_stride, k_head_stride;
+    const void* v;
+    uint64_t v_stride, v_head_stride;
+    uint64_t n_head_kv, hd, rot;
+    int layout;
+    const float* cos_t;
+    const float* sin_t;
+    uint64_t n_pos, n_rows;
+    KvRows rows;
+    void* k_pages;
+    void* v_pages;
+    void* k_scales;
+    void* v_scales;
+    int q_parts = 0;  // set by rope_kv_append
+};
+cudaError_t rope_kv_append(int type, const RopeAppendArgs& a, cudaStream_t s);
+struct KvReadArgs {
+    int kv_type;
+    const void* pages;
+    const void* scales;
+    uint64_t n_head_kv, hd;
+    KvRows rows;
+    void* out;  // [rows][n_head_kv][hd]
+};
+cudaError_t kv_read(int type, const KvReadArgs& a, uint64_t rows, cudaStream_t s);
+
+// ---- attn_q4.cu : attention over the 4-bit cache (kv_q4.cuh)
+struct AttnQ4Args {
+    const void* q;  // head h of row r at q + r * q_stride + h * hd
+    uint64_t q_stride;
+    uint64_t n_q, n_head, n_head_kv, hd;
+    const uint8_t* k_pages;
+    const uint8_t* v_pages;
+    const uint16_t* k_scales;
+    const uint16_t* v_scales;
+    const int32_t* block_table;  // [n_seq][max_pages]
+    uint64_t n_seq, max_pages, page, n_pages;
+    const int32_t* q_start;  // [n_seq + 1] first row of each sequence; nullptr: row r is sequence r
+    uint64_t max_q;          // most rows of one sequence
+    const int32_t* ctx_len;  // per row
+    uint64_t max_ctx;
+    float scale;
+    void* out;
+    uint64_t out_stride;
+};
+cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s);
+
 uint64_t attn_smem_bytes(uint64_t hd, uint64_t max_ctx, uint64_t max_pages, int kv_type);
 cudaError_t paged_attn_decode(const AttnArgs& a, cudaStream_t s);
 // attn_split.cu: the same, split over the context (warps merge their softmax
