@@ -510,8 +510,8 @@ int check_table(const int32_t* table, const int32_t* pos, uint64_t n_seq, uint64
     if (!table || !pos) return fail(MV_ERR_INVALID, "null block table or per-row array");
     if (!page || page > 0x7fffffffull) return fail(MV_ERR_INVALID, "page must be > 0");
     if (!n_seq || !max_pages) return fail(MV_ERR_INVALID, "the block table needs n_seq > 0 and max_pages > 0");
-    if (n_seq > 0x7fffffffull || n_pages > 0x7fffffffull || max_pages > 0x7fffffffull / page)
-        return fail(MV_ERR_INVALID, "max_pages * page, n_pages and n_seq must stay below 2^31");
+    if (n_seq > 0x7fffffffull || n_pages > 0x7fffffffull || max_pages > 0x7fff0000ull / page)
+        return fail(MV_ERR_INVALID, "max_pages * page (less 65536), n_pages and n_seq must stay below 2^31");
     return MV_OK;
 }
 // Attention calls: everything but the row layout.
@@ -631,6 +631,8 @@ MV_API int mv_paged_attn_q4(int type, const void* q, uint64_t q_row_stride, uint
         return rc;
     if (int rc = check_rows(n_seq, n_head, hd)) return rc;
     if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    if (n_pages * page >= 0xffffffffull / n_head_kv)
+        return fail(MV_ERR_INVALID, "the pool holds 2^32 or more (token, kv head) rows");
     mvb::AttnQ4Args a{q, q_row_stride, n_seq, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
                       static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
                       static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, nullptr, 1,
@@ -652,6 +654,8 @@ MV_API int mv_paged_attn_q4_prefill(int type, const void* q, uint64_t q_row_stri
         return rc;
     if (int rc = check_rows(n_q, n_head, hd)) return rc;
     if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    if (n_pages * page >= 0xffffffffull / n_head_kv)
+        return fail(MV_ERR_INVALID, "the pool holds 2^32 or more (token, kv head) rows");
     if (!q_start || !max_q || max_q > n_q) return fail(MV_ERR_INVALID, "prefill needs q_start and max_q in 1..n_q");
     mvb::AttnQ4Args a{q, q_row_stride, n_q, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
                       static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
