@@ -11,6 +11,7 @@
 
 #include "kernels.cuh"
 #include "kv_q4.cuh"
+#include "tc.cuh"
 
 namespace mvb {
 
@@ -101,8 +102,11 @@ cudaError_t attn_rows(const AttnQ4Args& a, cudaStream_t s) {
 // ------------------------------------------------------------- primitives
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // Asynchronous copies global -> shared; `bytes` 0 fills with zeros and reads nothing.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes) {
+__device__ __forceinline__ void cp_async_fill(uint32_t dst, const void* src, int bytes) {
     if constexpr (N == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
     else
@@ -156,22 +160,33 @@ __device__ __forceinline__ uint32_t nib_hi(uint32_t x) {
     const __half2 h = __hfma2(reinterpret_cast<const __half2&>(r), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
     return reinterpret_cast<const uint32_t&>(h);
 }
-// Nibbles 2 MU, 2 MU + 1 of x as n - 8 in fp32: each is masked in place and
-// ORed into the mantissa of 2^23, giving 2^23 + n 2^(4 i); one packed FMA
-// scales that back and takes 2^(23 - 4 i) + 8 off, exactly.
-template <int MU>
-__device__ __forceinline__ void nibbles2(uint32_t x, float& lo, float& hi) {
-    uint32_t u0, u1;
-    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u0) : "r"(x), "n"(0xf << (8 * MU)));
-    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u1) : "r"(x), "n"(0xf0 << (8 * MU)));
-    constexpr float m0 = MU ? 1.0f / 256 : 1.0f, m1 = m0 / 16;
-    constexpr float k0 = -(8388608.0f * m0 + 8.0f), k1 = -(8388608.0f * m1 + 8.0f);
-    uint64_t v, m, k;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(u0), "r"(u1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(m) : "f"(m0), "f"(m1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(k) : "f"(k0), "f"(k1));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(v), "l"(m), "l"(k));
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// Nibbles I, I + 1 of a token's word times its scale (twice in d): (n - 8) d in
+// fp32, exact (at most 11 bits).  A nibble is masked in place and ORed into
+// the mantissa of 2^23, giving 2^23 + n 2^(4 I); a packed FMA scales that back
+// and takes 2^(23 - 4 I) + 8 off.  The pair are neighbours in the MMA's A
+// registers (rows g, g + 8): pairs over two tokens cost a move each.
+template <int I>
+__device__ __forceinline__ void values2(uint32_t x, uint64_t d, float& v0, float& v1) {
+    uint32_t u0, u1;
+    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u0) : "r"(x), "n"(0xf << (4 * I)));
+    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u1) : "r"(x), "n"(0xf0 << (4 * I)));
+    constexpr float m = 1.0f / (1 << (4 * I)), k = 8388608.0f * m;
+    const uint64_t n = tc::f2_fma(pair(__uint_as_float(u0), __uint_as_float(u1)), pair(m, m / 16),
+                                  pair(-k - 8.0f, -k / 16 - 8.0f));
+    unpair(tc::f2_mul(n, d), v0, v1);
 }
 __device__ __forceinline__ float to_tf32(float x) {
     uint32_t r;
@@ -189,15 +204,15 @@ __device__ __forceinline__ float to_tf32(float x) {
 //  scores  (heads x tokens, m16n8k16 fp16): A = the queries, B = keys n - 8,
 //          exact; each 32-block's sum is multiplied by its scale afterwards, in
 //          fp32.
-//  outputs (dims x heads, m16n8k8 tf32): A = values n - 8, exact, B = the
-//          weights p d with the block's scale.  tf32 keeps the weights' whole
-//          exponent range: in fp16 a dimension whose heavy tokens are all zero
-//          lost the light ones.
+//  outputs (dims x heads, m16n8k8 tf32): A = the values (n - 8) d, exact in
+//          tf32's 11 bits, B = the weights.  tf32 keeps their whole exponent
+//          range: in fp16 a dimension whose heavy tokens are all zero lost the
+//          light ones.
 // fp32 queries and their weights go in as two parts of 11 bits: the queries'
 // second parts are rows 8..15 of A, the weights' are columns 4..7 for up to
 // four heads (PACK: rows 4..7 repeat heads 0..3, so a lane's weights are
 // already there) and a second MMA for more.
-constexpr int kWarps = 4, kStages = 3;
+constexpr int kWarps = 4, kStages = 3, kMaxSplits = 512;
 
 template <int HD>
 struct Q4Tile {
@@ -292,40 +307,47 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
     const int32_t* table = a.block_table + row * (int64_t)a.max_pages;
 
     // ---- copies.  Lane l looks the cache slots of tokens l (and l + 32) of a
-    // stage up; 0xffffffff: no such token.
-    auto slot_of = [&](int tok) -> uint32_t {
-        if (tok >= last) return 0xffffffffu;
-        const uint32_t pi = (uint32_t)(((uint64_t)(uint32_t)tok * sp.page_mul) >> sp.page_shift);
-        const int pg = table[pi];
-        if (pg < 0 || (uint64_t)pg >= a.n_pages) return 0xffffffffu;
-        return ((uint32_t)pg * (uint32_t)H + (uint32_t)kvh) * (uint32_t)a.page + ((uint32_t)tok - pi * (uint32_t)a.page);
-    };
-    constexpr int LT = TT > 32 ? TT / 32 : 1;  // tokens a lane looks up
-    uint32_t slots[LT];
+    // stage up; `exists` has a bit for each that is there.
+    constexpr int LT = TT > 32 ? TT / 32 : 1;
+    uint32_t slots[LT], exists;
     auto look_up = [&](int base) {
+        exists = 0;
 #pragma unroll
-        for (int i = 0; i < LT; ++i) slots[i] = lane + 32 * i < TT ? slot_of(base + lane + 32 * i) : 0xffffffffu;
+        for (int i = 0; i < LT; ++i) {
+            const uint32_t tok = (uint32_t)base + lane + 32 * i;
+            slots[i] = 0;
+            if (tok < (uint32_t)last && (TT >= 32 || lane < TT)) {
+                const uint32_t pi = (uint32_t)(((uint64_t)tok * sp.page_mul) >> sp.page_shift);
+                const uint32_t pg = (uint32_t)table[pi];
+                if (pg < (uint32_t)a.n_pages) {
+                    slots[i] = (pg * (uint32_t)H + (uint32_t)kvh) * (uint32_t)a.page + (tok - pi * (uint32_t)a.page);
+                    exists |= 1u << i;
+                }
+            }
+        }
     };
+    // a missing token's nibbles are those of slot 0 -- its scales are zeros and
+    // its score -inf -- so only the scale copies carry a size
+    const uint8_t* k_unit = a.k_pages + lane % X::U * 16;
+    const uint8_t* v_unit = a.v_pages + lane % X::U * 16;
     auto issue = [&](int s) {
         const uint32_t st = ring_s + s * X::kBytes;
 #pragma unroll
         for (int i = 0; i < 2048 / 16 / 32; ++i) {
-            const int c = i * 32 + lane, r = c / X::U, u = c % X::U;  // 16-byte unit u of token r
+            const int r = (i * 32 + lane) / X::U;  // unit lane % U of token r
             const uint32_t sl = __shfl_sync(0xffffffffu, slots[LT == 1 ? 0 : i * (32 / X::U) / 32], r & 31);
-            const uint64_t off = sl == 0xffffffffu ? 0 : (uint64_t)sl * (HD / 2) + u * 16;
-            const uint32_t dst = st + r * (HD / 2) + ((u ^ X::swz(r)) * 16);
-            const int n = sl == 0xffffffffu ? 0 : 16;
-            cp_async<16>(dst, a.k_pages + off, n);
-            cp_async<16>(dst + 2048, a.v_pages + off, n);
+            const uint32_t dst = st + r * (HD / 2) + ((lane % X::U ^ X::swz(r)) * 16);
+            cp_async16(dst, k_unit + (uint64_t)sl * (HD / 2));
+            cp_async16(dst + 2048, v_unit + (uint64_t)sl * (HD / 2));
         }
 #pragma unroll
         for (int i = 0; i < LT; ++i) {
-            const bool ok = slots[i] != 0xffffffffu;
+            const bool ok = exists >> i & 1u;
             if (TT >= 32 || lane < TT) {
-                const uint64_t off = ok ? (uint64_t)slots[i] * NB : 0;
+                const uint64_t off = (uint64_t)slots[i] * NB;
                 const uint32_t dst = st + 4096 + (lane + 32 * i) * (NB * 2);
-                cp_async<NB * 2>(dst, a.k_scales + off, ok ? NB * 2 : 0);
-                cp_async<NB * 2>(dst + X::kScale, a.v_scales + off, ok ? NB * 2 : 0);
+                cp_async_fill<NB * 2>(dst, a.k_scales + off, ok ? NB * 2 : 0);
+                cp_async_fill<NB * 2>(dst + X::kScale, a.v_scales + off, ok ? NB * 2 : 0);
             }
             const uint32_t v = __ballot_sync(0xffffffffu, ok);
             if (lane == 0) valid_ring[s * 2 + i] = v;
@@ -412,7 +434,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
             uint32_t w[NB], d[NB];
             load_words<HD>(w, kt, 8 * j + g, t);
             load_scales<HD>(d, ksc, 8 * j + 2 * t);
-            sc[j][0] = sc[j][1] = 0.0f;
+            uint64_t sum = 0;  // two zeros
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -427,10 +449,12 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
                     }
                     mma16816(c, qf, nib_lo(x), nib_hi(x), c);
                 }
-                if constexpr (kTwo) c[0] += c[2], c[1] += c[3];
-                sc[j][0] = fmaf(c[0], scale_of<HD>(d, 0, b), sc[j][0]);
-                sc[j][1] = fmaf(c[1], scale_of<HD>(d, 1, b), sc[j][1]);
+                const uint64_t dd = pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b));
+                uint64_t cc = pair(c[0], c[1]);
+                if constexpr (kTwo) cc = f2_add(cc, pair(c[2], c[3]));
+                sum = tc::f2_fma(cc, dd, sum);
             }
+            unpair(sum, sc[j][0], sc[j][1]);
         }
         // tokens that do not exist
 #pragma unroll
@@ -470,7 +494,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
         const int half = (g & 1) * 16;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            float p[2];
+            float p[2], r[2];
             uint32_t d[NB], w[2][NB];
             load_scales<HD>(d, vsc, 8 * j + 2 * t);
 #pragma unroll
@@ -478,38 +502,28 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
                 p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
                 l_run += p[i];
                 load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
+                if constexpr (kTwo) {
+                    const float hi = __uint_as_float(__float_as_uint(p[i]) & 0xffffe000u);  // 11 bits
+                    r[i] = p[i] - hi;
+                    p[i] = PACK && g >= 4 ? r[i] : hi;
+                } else {
+                    p[i] = to_tf32(p[i]);
+                }
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float v[2] = {p[0] * scale_of<HD>(d, 0, b), p[1] * scale_of<HD>(d, 1, b)};
+                const float dA = scale_of<HD>(d, 0, b), dB = scale_of<HD>(d, 1, b);
                 const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
-                float f0[4], f1[4];
-                nibbles2<0>(x0, f0[0], f0[1]);
-                nibbles2<0>(x1, f0[2], f0[3]);
-                nibbles2<1>(x0, f1[0], f1[1]);
-                nibbles2<1>(x1, f1[2], f1[3]);
-                if constexpr (!kTwo) {
-                    v[0] = to_tf32(v[0]), v[1] = to_tf32(v[1]);
-                    mma1688(o[b][0], f0, v[0], v[1]);
-                    mma1688(o[b][1], f1, v[0], v[1]);
-                } else {
-                    float r[2];  // what the first 11 bits leave
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float hi = __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
-                        r[i] = v[i] - hi;
-                        v[i] = hi;
-                    }
-                    if constexpr (PACK) {
-                        if (g >= 4) v[0] = r[0], v[1] = r[1];
-                        mma1688(o[b][0], f0, v[0], v[1]);
-                        mma1688(o[b][1], f1, v[0], v[1]);
-                    } else {
-                        mma1688(o[b][0], f0, v[0], v[1]);
-                        mma1688(o[b][1], f1, v[0], v[1]);
-                        mma1688(o[b][0], f0, r[0], r[1]);
-                        mma1688(o[b][1], f1, r[0], r[1]);
-                    }
+                float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
+                values2<0>(x0, pair(dA, dA), f0[0], f0[1]);
+                values2<0>(x1, pair(dB, dB), f0[2], f0[3]);
+                values2<2>(x0, pair(dA, dA), f1[0], f1[1]);
+                values2<2>(x1, pair(dB, dB), f1[2], f1[3]);
+                mma1688(o[b][0], f0, p[0], p[1]);
+                mma1688(o[b][1], f1, p[0], p[1]);
+                if constexpr (kTwo && !PACK) {
+                    mma1688(o[b][0], f0, r[0], r[1]);
+                    mma1688(o[b][1], f1, r[0], r[1]);
                 }
             }
         }
@@ -522,6 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
         cp_async_commit();
         s = s + 1 == kStages ? 0 : s + 1;
     }
+    pdl_trigger();  // the join may be set up
     cp_async_wait<0>();
     __syncthreads();  // the ring is reused for the warps' results
 
@@ -601,30 +616,55 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
     }
 }
 
-// Joins the parts of one unit (a CTA each): out = sum_r 2^(m_r - m) o_r / sum_r 2^(m_r - m) l_r.
+// Joins the parts of one unit's head (a CTA each): out = sum_r 2^(m_r - m) o_r
+// / sum_r 2^(m_r - m) l_r, the parts dealt to groups of HD / 4 threads.
 template <class T, int HD>
 __global__ void __launch_bounds__(256) attn_q4_join_kernel(AttnQ4Args a, Q4Split sp) {
+    constexpr int kLane = HD / 4, kGroups = 256 / kLane;
+    __shared__ float c[kMaxSplits], red[kGroups][HD + 1];
     const int64_t unit = blockIdx.x;
-    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, hs = sp.heads;
+    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, hs = sp.heads, h = blockIdx.y;
     const int chunk = (int)(unit % sp.chunks), kvh = (int)(unit / sp.chunks % H);
     const int64_t row = unit / sp.chunks / H;
-    const int h0 = kvh * G + chunk * hs, nh = min(hs, G - chunk * hs);
+    if (chunk * hs + h >= G) return;
     const int ctx = (int)max(0, min(a.ctx_len[row], (int)a.max_ctx));
     const int per = q4_part(ctx, sp.splits, kWarps * Q4Tile<HD>::TT), parts = per ? (ctx + per - 1) / per : 0;
     const int64_t stride = (int64_t)hs * (HD + 2);
     const float* src = sp.scratch + unit * sp.splits * stride;
-    T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)h0 * HD;
-    for (int i = threadIdx.x; i < nh * HD; i += 256) {
-        const int h = i / HD;
-        float mt = -INFINITY, y = 0.0f, l = 0.0f;
-        for (int r = 0; r < parts; ++r) mt = fmaxf(mt, src[r * stride + hs * HD + h]);
-        for (int r = 0; r < parts; ++r) {
-            const float* p = src + r * stride;
-            const float m = p[hs * HD + h], c = m == -INFINITY ? 0.0f : ex2(m - mt);
-            y = fmaf(c, p[i], y);
-            l = fmaf(c, p[hs * (HD + 1) + h], l);
-        }
-        out[i] = from_f32<T>(l == 0.0f ? 0.0f : y / l);
+    pdl_wait();
+    float mt = -INFINITY, l = 0.0f;
+    for (int r = threadIdx.x; r < parts; r += 256) mt = fmaxf(mt, src[r * stride + hs * HD + h]);
+    mt = warp_max(mt);
+    if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = mt;
+    __syncthreads();
+    mt = red[0][0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) mt = fmaxf(mt, red[0][w]);
+    for (int r = threadIdx.x; r < parts; r += 256) {
+        const float m = src[r * stride + hs * HD + h];
+        c[r] = m == -INFINITY ? 0.0f : ex2(m - mt);
+    }
+    __syncthreads();
+    const int d = threadIdx.x % kLane * 4, grp = threadIdx.x / kLane;
+    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = grp; r < parts; r += kGroups) {
+        const float w = c[r];
+        const float2 u = *reinterpret_cast<const float2*>(src + r * stride + h * HD + d),
+                     v = *reinterpret_cast<const float2*>(src + r * stride + h * HD + d + 2);
+        y[0] = fmaf(w, u.x, y[0]), y[1] = fmaf(w, u.y, y[1]);
+        y[2] = fmaf(w, v.x, y[2]), y[3] = fmaf(w, v.y, y[3]);
+        if (d == 0) l = fmaf(w, src[r * stride + hs * (HD + 1) + h], l);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[grp][d + i] = y[i];
+    if (d == 0) red[grp][HD] = l;
+    __syncthreads();
+    T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)(kvh * G + chunk * hs + h) * HD;
+    for (int i = threadIdx.x; i < HD; i += 256) {
+        float v = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kGroups; ++w) v += red[w][i], den += red[w][HD];
+        out[i] = from_f32<T>(den == 0.0f ? 0.0f : v / den);
     }
 }
 
@@ -636,6 +676,13 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     const int smem = std::max(kWarps * X::kRing + kWarps * kStages * 8, merge);
     auto kernel = attn_q4_decode_kernel<T, HD, PACK>;
     ensure_smem_attr(kernel, smem);
+    static const int slots = [&] {  // CTAs that the GPU holds at once
+        int per = 0, sms = 0, dev = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kWarps * 32, smem);
+        return std::max(1, per * sms);
+    }();
     Q4Split sp{};
     const uint64_t G = a.n_head / a.n_head_kv;
     sp.chunks = (int)((G + kHeads - 1) / kHeads);
@@ -644,12 +691,12 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     while ((1ull << L) < a.page) ++L;
     sp.page_mul = (uint32_t)(((1ull << (31 + L)) + a.page - 1) / a.page);
     sp.page_shift = 31 + L;
-    // enough CTAs for three on every SM, none with less than one stage per warp,
+    // enough CTAs to fill the GPU once, none with less than one stage per warp,
     // and none with more than 2048 tokens (a long sequence among short ones
     // would otherwise keep one CTA busy after the others are done)
     const uint64_t stages = (a.max_ctx + kCta - 1) / kCta;
-    uint64_t want = std::max<uint64_t>((444 + units - 1) / units, (a.max_ctx + 2047) / 2048);
-    want = std::max<uint64_t>(1, std::min<uint64_t>({want, stages, 512}));
+    uint64_t want = std::max<uint64_t>(slots / units, (a.max_ctx + 2047) / 2048);
+    want = std::max<uint64_t>(1, std::min<uint64_t>({want, stages, kMaxSplits}));
     sp.heads = (int)std::min<uint64_t>(kHeads, G);
     if (units * want > 0x7fffffffull) return cudaErrorInvalidConfiguration;
     if (want > 1 && want <= 8) {  // a cluster
@@ -671,6 +718,7 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
         return cudaLaunchKernelEx(&cfg, kernel, a, sp);
     }
     sp.splits = (int)want;
+    if (want > 1) keep_pool_memory();
     if (want > 1)
         if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&sp.scratch), units * want * sp.heads * (HD + 2) * 4, s))
             return e;
@@ -678,8 +726,7 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (want > 1) {
         if (e == cudaSuccess) {
-            attn_q4_join_kernel<T, HD><<<(unsigned)units, 256, 0, s>>>(a, sp);
-            e = cudaGetLastError();
+            e = launch_pdl(attn_q4_join_kernel<T, HD>, dim3((unsigned)units, (unsigned)sp.heads), dim3(256), 0, s, a, sp);
         }
         cudaFreeAsync(sp.scratch, s);
     }

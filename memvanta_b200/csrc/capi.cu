@@ -12,6 +12,7 @@
 #include <string>
 
 #include "../../include/memvanta_b200.h"
+#include "common.cuh"
 #include "kernels.cuh"
 #include "weights.cuh"
 
@@ -90,17 +91,6 @@ struct HostCallBuffers {
 HostCallBuffers& host_buffers() {
     static thread_local HostCallBuffers b;
     return b;
-}
-
-// Stream-ordered scratch (cudaMallocAsync) comes from the device's default
-// pool; keep freed blocks in the pool instead of returning them to the driver
-// at every synchronisation.
-void keep_pool_memory(int device) {
-    cudaMemPool_t pool;
-    if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
-        uint64_t threshold = UINT64_MAX;
-        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
-    }
 }
 
 int check_weight(const mv_weight_s* w) {
@@ -232,7 +222,7 @@ MV_API int mv_init(int device) {
     if (major != 10)
         return fail(MV_ERR_UNSUPPORTED, "memvanta_b200 is built for sm_100a; device has compute capability " +
                                             std::to_string(major) + ".x");
-    keep_pool_memory(device);
+    mvb::keep_pool_memory();
     return MV_OK;
 }
 
@@ -631,6 +621,7 @@ MV_API int mv_paged_attn_q4(int type, const void* q, uint64_t q_row_stride, uint
         return rc;
     if (int rc = check_rows(n_seq, n_head, hd)) return rc;
     if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    if (!n_pages) return fail(MV_ERR_INVALID, "the cache has no pages");
     if (n_pages * page >= 0xffffffffull / n_head_kv)
         return fail(MV_ERR_INVALID, "the pool holds 2^32 or more (token, kv head) rows");
     mvb::AttnQ4Args a{q, q_row_stride, n_seq, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
@@ -654,6 +645,7 @@ MV_API int mv_paged_attn_q4_prefill(int type, const void* q, uint64_t q_row_stri
         return rc;
     if (int rc = check_rows(n_q, n_head, hd)) return rc;
     if (int rc = check_table(block_table, ctx_len, n_seq, max_pages, page, n_pages)) return rc;
+    if (!n_pages) return fail(MV_ERR_INVALID, "the cache has no pages");
     if (n_pages * page >= 0xffffffffull / n_head_kv)
         return fail(MV_ERR_INVALID, "the pool holds 2^32 or more (token, kv head) rows");
     if (!q_start || !max_q || max_q > n_q) return fail(MV_ERR_INVALID, "prefill needs q_start and max_q in 1..n_q");

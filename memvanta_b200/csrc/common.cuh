@@ -25,6 +25,23 @@ inline void ensure_smem_attr(Kernel* k, int bytes) {
     done.insert(key);
 }
 
+// Stream-ordered scratch (cudaMallocAsync) comes from the current device's
+// default pool; keep freed blocks in the pool instead of returning them to the
+// driver at every synchronisation.  Set once per device.
+inline void keep_pool_memory() {
+    static std::mutex mu;
+    static std::set<int> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (!done.insert(dev).second) return;
+    cudaMemPool_t pool;
+    if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess) {
+        uint64_t threshold = UINT64_MAX;
+        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
+    }
+}
+
 // ------------------------------------------------- programmatic launches
 // Programmatic dependent launch: a kernel launched with launch_pdl may start
 // while the previous kernel in the stream is still running.  It must call
