@@ -4,7 +4,6 @@
 // over the first ctx_len[r] cached tokens of the row's sequence, in one pass
 // with the running maximum m and sum.  A row with no tokens gives zeros; what
 // lies past ctx_len, or on a page that does not exist, is never used.
-#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -14,8 +13,6 @@
 #include "tc.cuh"
 
 namespace mvb {
-
-namespace cg = cooperative_groups;
 
 namespace {
 
@@ -144,10 +141,10 @@ __device__ __forceinline__ void mma1688(float (&d)[4], const float (&a)[4], floa
         : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
           "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
-// Nibbles 0 and 4 (lo), or 1 and 5 (hi), of x as two fp16 numbers n - 8: ORed
-// into 1024 they are 1024 + n, or 1024 + 16 n, and one fp16 operation is exact.
-// (As fp16 subnormals n 2^-24, without that operation, the tensor core aligned
-// its sum to their exponent field, 2^-14, and scores lost 4 bits.)
+// Nibbles 0 and 4 of x as the fp16 numbers n - 8, or nibbles 1 and 5 as 16 (n -
+// 8): ORed into 1024 they are 1024 + n, or 1024 + 16 n, and one subtraction is
+// exact.  (As fp16 subnormals n 2^-24, without it, the tensor core aligned its
+// sum to their exponent field, 2^-14, and scores lost 4 bits.)
 __device__ __forceinline__ uint32_t nib_lo(uint32_t x) {
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(x));
@@ -157,7 +154,7 @@ __device__ __forceinline__ uint32_t nib_lo(uint32_t x) {
 __device__ __forceinline__ uint32_t nib_hi(uint32_t x) {
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(x));
-    const __half2 h = __hfma2(reinterpret_cast<const __half2&>(r), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
+    const __half2 h = __hadd2(reinterpret_cast<const __half2&>(r), __float2half2_rn(-1152.0f));
     return reinterpret_cast<const uint32_t&>(h);
 }
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -173,46 +170,50 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 __device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
-// Nibbles I, I + 1 of a token's word times its scale (twice in d): (n - 8) d in
-// fp32, exact (at most 11 bits).  A nibble is masked in place and ORed into
-// the mantissa of 2^23, giving 2^23 + n 2^(4 I); a packed FMA scales that back
-// and takes 2^(23 - 4 I) + 8 off.  The pair are neighbours in the MMA's A
-// registers (rows g, g + 8): pairs over two tokens cost a move each.
+// Nibbles I, I + 1 of x as (n - 8) 16^I, (n - 8) 16^(I + 1) in fp32: each is
+// masked in place and ORed into the mantissa of 2^23, and one packed addition
+// takes `bias`, the pair 2^23 + 8 16^I, .., off.  The pair are neighbours in
+// the MMA's A registers (rows g, g + 8).
 template <int I>
-__device__ __forceinline__ void values2(uint32_t x, uint64_t d, float& v0, float& v1) {
+__device__ __forceinline__ void values2(uint32_t x, uint64_t bias, float& v0, float& v1) {
     uint32_t u0, u1;
     asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u0) : "r"(x), "n"(0xf << (4 * I)));
     asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u1) : "r"(x), "n"(0xf0 << (4 * I)));
-    constexpr float m = 1.0f / (1 << (4 * I)), k = 8388608.0f * m;
-    const uint64_t n = tc::f2_fma(pair(__uint_as_float(u0), __uint_as_float(u1)), pair(m, m / 16),
-                                  pair(-k - 8.0f, -k / 16 - 8.0f));
-    unpair(tc::f2_mul(n, d), v0, v1);
+    unpair(f2_add(pair(__uint_as_float(u0), __uint_as_float(u1)), bias), v0, v1);
 }
-__device__ __forceinline__ float to_tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return __uint_as_float(r);
+// A pair of constants that stays in registers (the compiler would build it anew at every use).
+__device__ __forceinline__ uint64_t held_pair(float lo, float hi) {
+    uint64_t r;
+    asm volatile("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
 
 // ---------------------------------------------------------- one query row
-// A CTA of 4 warps takes one (sequence, kv head, up to 8 of its query heads)
-// and a range of tokens; each warp its own 4096 / HD tokens of every fourth
-// part of the range ("a stage"), through a ring of its own in shared memory
-// (cp.async; no barrier between warps until the end).
+// The work is a row of stages -- 4096 / HD tokens of one unit (a query row, a
+// kv head, up to 8 of its query heads) -- cut into equal runs, one for each
+// warp that the GPU holds at once, whatever the contexts' lengths.  A warp
+// streams its run through a ring of its own in shared memory (cp.async; no
+// barrier after the start) and goes from unit to unit without draining it.  A
+// unit inside one run is written out by its warp; the parts of the others go to
+// scratch and are joined by a second kernel.
 //
 // Both products run on the tensor cores, the cache as integers:
 //  scores  (heads x tokens, m16n8k16 fp16): A = the queries, B = keys n - 8,
 //          exact; each 32-block's sum is multiplied by its scale afterwards, in
 //          fp32.
-//  outputs (dims x heads, m16n8k8 tf32): A = the values (n - 8) d, exact in
-//          tf32's 11 bits, B = the weights.  tf32 keeps their whole exponent
+//  outputs (dims x heads, m16n8k8 tf32): A = values (n - 8) 16^i, exact, the
+//          power of the nibble's place taken off at the end; B = the weights p d
+//          with the block's scale.  tf32 keeps the weights' whole exponent
 //          range: in fp16 a dimension whose heavy tokens are all zero lost the
 //          light ones.
 // fp32 queries and their weights go in as two parts of 11 bits: the queries'
 // second parts are rows 8..15 of A, the weights' are columns 4..7 for up to
 // four heads (PACK: rows 4..7 repeat heads 0..3, so a lane's weights are
-// already there) and a second MMA for more.
-constexpr int kWarps = 4, kStages = 3, kMaxSplits = 512;
+// already there) and a second MMA for more.  The tensor core ignores the low
+// 13 bits of a tf32 operand, so the first part needs no masking; half-precision
+// queries' weights go in as one part, and p carries a factor 1 + 2^-12 that
+// makes up for what that cut takes off on average.
+constexpr int kWarps = 4, kStages = 3;
 
 template <int HD>
 struct Q4Tile {
@@ -228,20 +229,29 @@ struct Q4Tile {
     static __device__ __forceinline__ int swz(int r) { return (r >> (U == 8 ? 0 : U == 4 ? 1 : 2)) & (U - 1); }
 };
 
-struct Q4Split {       // how a launch cuts the tokens
-    int splits;        // CTAs per unit: a cluster, or with scratch any number
-    float* scratch;    // [units][splits][heads][HD + 2] or nullptr
+struct Q4Split {
+    float* scratch;    // parts: [2 * warps][heads][HD], then their maxima and sums [2 * warps][heads][2]
+    int4* joins;       // per unit, or per warp where the units are more: {unit, first part, its warp, last warp or -1}
+    int by_unit;
     int heads;         // query heads of a unit at most
-    int chunks;        // query-head chunks of 8 (4 with PACK) per kv head
+    int chunks;        // units per kv head
     uint32_t page_mul; // t / page = t * page_mul >> page_shift for t < 2^31
     int page_shift;
 };
 
-// Tokens of each part of a context: equal, in whole CTA stages, so a short
-// context takes fewer parts than there are.
-__device__ __forceinline__ int q4_part(int ctx, int splits, int stage) {
-    return ((ctx + splits - 1) / splits + stage - 1) / stage * stage;
+// Stages of a query row's context, per unit.
+template <int HD>
+__device__ __forceinline__ int q4_stages(const AttnQ4Args& a, int64_t row) {
+    const int ctx = max(0, min(a.ctx_len[row], (int)a.max_ctx));
+    return (ctx + Q4Tile<HD>::TT - 1) / Q4Tile<HD>::TT;
 }
+
+// A place in the row of stages.
+struct Q4Place {
+    int row, kvh, chunk;
+    int stage, stages;  // of this unit
+    int ctx;
+};
 
 // words b = 0 .. NB - 1 at 32-bit word t * NB + b of a swizzled row
 template <int HD>
@@ -283,44 +293,98 @@ __device__ __forceinline__ float scale_of(const uint32_t (&s)[HD / 32], int k, i
 }
 
 template <class T, int HD, bool PACK>
-__global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args a, Q4Split sp) {
+__global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode_kernel(AttnQ4Args a, Q4Split sp) {
     using X = Q4Tile<HD>;
     constexpr int TT = X::TT, NB = X::NB, NJ = X::NJ;
     constexpr bool kTwo = sizeof(T) == 4;  // two fp16 parts
     static_assert(!PACK || kTwo, "packing is for two parts");
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv;
-    const int split = (int)blockIdx.x % sp.splits;
-    const int64_t unit = blockIdx.x / (unsigned)sp.splits;  // (row, kv head, chunk of heads)
-    const int chunk = (int)(unit % sp.chunks), kvh = (int)(unit / sp.chunks % H);
-    const int64_t row = unit / sp.chunks / H;
-    const int h0 = kvh * G + chunk * sp.heads, nh = min(sp.heads, G - chunk * sp.heads);
-    const int ctx = (int)max(0, min(a.ctx_len[row], (int)a.max_ctx));
-    const int per = q4_part(ctx, sp.splits, kWarps * TT);
-    const int first = (int)min((int64_t)ctx, (int64_t)split * per), last = (int)min((int64_t)ctx, (int64_t)first + per);
-    if (sp.scratch && first >= last) return;
+    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, upr = H * sp.chunks;
+
+    pdl_trigger();  // the join may be set up as soon as there is room
+    // ---- this warp's run of stages.  Thread i sums the stages of rows i R ..
+    // i R + R - 1; the warp finds the thread, then the row, where its run starts.
+    const int64_t n_row = (int64_t)a.n_q, R = (n_row + kWarps * 32 - 1) / (kWarps * 32);
+    int64_t* before = reinterpret_cast<int64_t*>(smem);  // [129], in the ring's place
+    int64_t mine = 0;
+    for (int64_t r = threadIdx.x * R; r < min(n_row, (threadIdx.x + 1) * R); ++r) mine += q4_stages<HD>(a, r);
+    int64_t upto = mine;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, k);
+        if (lane >= k) upto += x;
+    }
+    if (lane == 31) before[kWarps * 32 + 1 + warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += before[kWarps * 32 + 1 + w];
+    before[threadIdx.x + 1] = upto;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    const int64_t total = before[kWarps * 32] * upr;
+    // warp numbers run over the CTAs first, so that few stages spread over all SMs
+    const int64_t W = min((int64_t)gridDim.x * kWarps, total), wid = (int64_t)warp * gridDim.x + blockIdx.x;
+    const int64_t s0 = wid < W ? wid * total / W : 0, s1 = wid < W ? (wid + 1) * total / W : 0;
+    Q4Place at{0, 0, 0, 0, 1, 0};
+    if (s0 < s1) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) n += __popc(__ballot_sync(0xffffffffu, before[k * 32 + lane] * upr <= s0));
+        int64_t rest = s0 - before[n - 1] * upr;
+        at.row = (int)((n - 1) * R);
+        while (true) {
+            at.stages = q4_stages<HD>(a, at.row);
+            if (rest < (int64_t)at.stages * upr) break;
+            rest -= (int64_t)at.stages * upr;
+            ++at.row;
+        }
+        const int u = (int)(rest / at.stages);
+        at.stage = (int)(rest - (int64_t)u * at.stages);
+        at.kvh = u / sp.chunks;
+        at.chunk = u % sp.chunks;
+        at.ctx = min(a.ctx_len[at.row], (int)a.max_ctx);
+    }
+    __syncthreads();  // `before` has been read
+    // rows with no tokens give zeros
+    for (int64_t r = blockIdx.x; r < n_row; r += gridDim.x)
+        if (min(a.ctx_len[r], (int)a.max_ctx) <= 0)
+            for (int i = threadIdx.x; i < (int)a.n_head * HD; i += kWarps * 32)
+                static_cast<T*>(a.out)[r * (int64_t)a.out_stride + i] = from_f32<T>(0.0f);
+    if (!sp.by_unit && lane == 0) sp.joins[(int64_t)warp * gridDim.x + blockIdx.x].w = -1;
+    if (s0 >= s1) return;
+    auto next = [&](Q4Place& p) {
+        if (++p.stage < p.stages) return;
+        p.stage = 0;
+        if (++p.chunk < sp.chunks) return;
+        p.chunk = 0;
+        if (++p.kvh < H) return;
+        p.kvh = 0;
+        do {
+            if (++p.row >= n_row) return;
+            p.stages = q4_stages<HD>(a, p.row);
+        } while (p.stages == 0);
+        p.ctx = min(a.ctx_len[p.row], (int)a.max_ctx);
+    };
 
     uint8_t* ring = smem + warp * X::kRing;
     const uint32_t ring_s = smem_u32(ring);
     uint32_t* valid_ring = reinterpret_cast<uint32_t*>(smem + kWarps * X::kRing) + warp * kStages * 2;
-    const int32_t* table = a.block_table + row * (int64_t)a.max_pages;
 
     // ---- copies.  Lane l looks the cache slots of tokens l (and l + 32) of a
     // stage up; `exists` has a bit for each that is there.
     constexpr int LT = TT > 32 ? TT / 32 : 1;
     uint32_t slots[LT], exists;
-    auto look_up = [&](int base) {
+    auto look_up = [&](const Q4Place& p) {
         exists = 0;
 #pragma unroll
         for (int i = 0; i < LT; ++i) {
-            const uint32_t tok = (uint32_t)base + lane + 32 * i;
+            const uint32_t tok = (uint32_t)p.stage * TT + lane + 32 * i;
             slots[i] = 0;
-            if (tok < (uint32_t)last && (TT >= 32 || lane < TT)) {
+            if (tok < (uint32_t)p.ctx && (TT >= 32 || lane < TT)) {
                 const uint32_t pi = (uint32_t)(((uint64_t)tok * sp.page_mul) >> sp.page_shift);
-                const uint32_t pg = (uint32_t)table[pi];
+                const uint32_t pg = (uint32_t)a.block_table[(int64_t)p.row * (int64_t)a.max_pages + pi];
                 if (pg < (uint32_t)a.n_pages) {
-                    slots[i] = (pg * (uint32_t)H + (uint32_t)kvh) * (uint32_t)a.page + (tok - pi * (uint32_t)a.page);
+                    slots[i] = (pg * (uint32_t)H + (uint32_t)p.kvh) * (uint32_t)a.page + (tok - pi * (uint32_t)a.page);
                     exists |= 1u << i;
                 }
             }
@@ -353,73 +417,86 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
             if (lane == 0) valid_ring[s * 2 + i] = v;
         }
     };
-    const int base0 = first + warp * TT;
-    constexpr int kStep = kWarps * TT;
+    Q4Place ahead = at;
+    int left = (int)(s1 - s0);  // stages to copy
+    look_up(ahead);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
-        if (base0 + s * kStep < last) {
-            look_up(base0 + s * kStep);
+        if (left > 0) {
             issue(s);
+            if (--left) next(ahead), look_up(ahead);
         }
         cp_async_commit();
     }
-    look_up(base0 + (kStages - 1) * kStep);
 
     // ---- the queries as A fragments.  Row g of the fragment is query head
     // hrow; k slots 2t, 2t + 1, 2t + 8, 2t + 9 of step s of block b are
-    // dimensions 32 b + 8 t + {0, 4, 1, 5} + 2 s.
+    // dimensions 32 b + 8 t + {0, 4, 1, 5} + 2 s, the last two divided by 16.
     const int hrow = PACK ? (g & 3) : g;
     uint32_t qa[NB][2][kTwo ? 4 : 2];
     float c_h;
-    {
-        const T* q = static_cast<const T*>(a.q) + row * (int64_t)a.q_stride + (int64_t)(h0 + min(hrow, nh - 1)) * HD;
-        float x[NB][8], mx = 0.0f;
+    int h0, nh;
+
+    const uint64_t bias0 = held_pair(-8388616.0f, -8388736.0f), bias1 = held_pair(-8390656.0f, -8421376.0f);
+    const uint32_t first = g >= 4 ? 0xffffe000u : 0u;
+    float o[NB][2][4];  // [block][dims 4g + 2 mu + {0, 1}][heads 2t, 2t + 1 of rows g, g + 8]
+    float m_run = -INFINITY, l_run = 0.0f;
+    const int count = (int)(s1 - s0);
+    int start = 0, start_stage = at.stage;  // where this warp's part of the unit begins, and its stage there
+    bool fresh = true;
+    int s = 0;
+    for (int n = 0; n < count; ++n) {
+        if (fresh) {
+            h0 = at.kvh * G + at.chunk * sp.heads;
+            nh = min(sp.heads, G - at.chunk * sp.heads);
+            const T* q = static_cast<const T*>(a.q) + (int64_t)at.row * (int64_t)a.q_stride + (int64_t)(h0 + min(hrow, nh - 1)) * HD;
+            float x[NB][8], mx = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            load_n<8, true>(q + 32 * b + 8 * t, x[b]);
+            for (int b = 0; b < NB; ++b) {
+                load_n<8, true>(q + 32 * b + 8 * t, x[b]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[b][i]));
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // times 2^e: the largest below 2^15
-        const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
-        const float up = pow2i(e);
-        c_h = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
+                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[b][i]));
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // times 2^e: the largest below 2^15
+            const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+            const float up = pow2i(e);
+            c_h = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[b][i] *= up;
+                for (int i = 0; i < 8; ++i) x[b][i] *= up;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const float f[4] = {x[b][2 * s], x[b][2 * s + 4], x[b][2 * s + 1], x[b][2 * s + 5]};
-                float lo[4];
+                for (int s = 0; s < 2; ++s) {
+                    const float f[4] = {x[b][2 * s], x[b][2 * s + 4], x[b][2 * s + 1] * 0.0625f,
+                                        x[b][2 * s + 5] * 0.0625f};
+                    float lo[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lo[i] = f[i] - __half2float(__float2half_rn(f[i]));
-                if constexpr (kTwo) {
-                    qa[b][s][0] = pack_half2(f[0], f[1]);
-                    qa[b][s][1] = pack_half2(lo[0], lo[1]);
-                    qa[b][s][2] = pack_half2(f[2], f[3]);
-                    qa[b][s][3] = pack_half2(lo[2], lo[3]);
-                } else {
-                    qa[b][s][0] = pack_half2(f[0], f[1]);
-                    qa[b][s][1] = pack_half2(f[2], f[3]);
+                    for (int i = 0; i < 4; ++i) lo[i] = f[i] - __half2float(__float2half_rn(f[i]));
+                    if constexpr (kTwo) {
+                        qa[b][s][0] = pack_half2(f[0], f[1]);
+                        qa[b][s][1] = pack_half2(lo[0], lo[1]);
+                        qa[b][s][2] = pack_half2(f[2], f[3]);
+                        qa[b][s][3] = pack_half2(lo[2], lo[3]);
+                    } else {
+                        qa[b][s][0] = pack_half2(f[0], f[1]);
+                        qa[b][s][1] = pack_half2(f[2], f[3]);
+                    }
                 }
             }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
+            m_run = -INFINITY;
+            l_run = 0.0f;
+            start = n;
+            start_stage = at.stage;
+            fresh = false;
         }
-    }
-
-    float o[NB][2][4];  // [block][dims 4g + 2 mu + {0, 1}][heads 2t, 2t + 1 of rows g, g + 8]
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
-
-    int s = 0;
-    for (int base = base0; base < last; base += kStep) {
         cp_async_wait<kStages - 2>();
         __syncwarp();
         const uint8_t* kt = ring + s * X::kBytes;
@@ -494,242 +571,223 @@ __global__ void __launch_bounds__(kWarps * 32) attn_q4_decode_kernel(AttnQ4Args 
         const int half = (g & 1) * 16;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            float p[2], r[2];
+            float p[2];
             uint32_t d[NB], w[2][NB];
             load_scales<HD>(d, vsc, 8 * j + 2 * t);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
                 l_run += p[i];
+                if constexpr (!kTwo) p[i] *= 1.000244140625f;
                 load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
-                if constexpr (kTwo) {
-                    const float hi = __uint_as_float(__float_as_uint(p[i]) & 0xffffe000u);  // 11 bits
-                    r[i] = p[i] - hi;
-                    p[i] = PACK && g >= 4 ? r[i] : hi;
-                } else {
-                    p[i] = to_tf32(p[i]);
-                }
             }
+            const uint64_t pp = pair(p[0], p[1]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float dA = scale_of<HD>(d, 0, b), dB = scale_of<HD>(d, 1, b);
+                float v[2];
+                const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
+                unpair(vv, v[0], v[1]);
                 const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
                 float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
-                values2<0>(x0, pair(dA, dA), f0[0], f0[1]);
-                values2<0>(x1, pair(dB, dB), f0[2], f0[3]);
-                values2<2>(x0, pair(dA, dA), f1[0], f1[1]);
-                values2<2>(x1, pair(dB, dB), f1[2], f1[3]);
-                mma1688(o[b][0], f0, p[0], p[1]);
-                mma1688(o[b][1], f1, p[0], p[1]);
+                values2<0>(x0, bias0, f0[0], f0[1]);
+                values2<0>(x1, bias0, f0[2], f0[3]);
+                values2<2>(x0, bias1, f1[0], f1[1]);
+                values2<2>(x1, bias1, f1[2], f1[3]);
+                if constexpr (PACK) {
+                    // columns 0..3: v, cut to 11 bits by the MMA; 4..7: v less its first 11 bits
+                    const uint64_t cut = pair(-__uint_as_float(__float_as_uint(v[0]) & first),
+                                              -__uint_as_float(__float_as_uint(v[1]) & first));
+                    unpair(f2_add(vv, cut), v[0], v[1]);
+                }
+                mma1688(o[b][0], f0, v[0], v[1]);
+                mma1688(o[b][1], f1, v[0], v[1]);
                 if constexpr (kTwo && !PACK) {
-                    mma1688(o[b][0], f0, r[0], r[1]);
-                    mma1688(o[b][1], f1, r[0], r[1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
+                    mma1688(o[b][0], f0, v[0], v[1]);
+                    mma1688(o[b][1], f1, v[0], v[1]);
                 }
             }
         }
         // ---- the next copies, into the stage used before this one
         __syncwarp();
-        if (base + (kStages - 1) * kStep < last) {
+        if (left > 0) {
             issue((s + kStages - 1) % kStages);
-            look_up(base + kStages * kStep);
+            if (--left) next(ahead), look_up(ahead);
         }
         cp_async_commit();
         s = s + 1 == kStages ? 0 : s + 1;
-    }
-    pdl_trigger();  // the join may be set up
-    cp_async_wait<0>();
-    __syncthreads();  // the ring is reused for the warps' results
 
-    // ---- the warps' results, then the CTA's
-    float* po = reinterpret_cast<float*>(smem);      // [warp][8 heads][HD]
-    float* pm = po + kWarps * 8 * HD;                // [warp][8] maxima, sums
-    float* pl = pm + kWarps * 8;
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    if (t == 0) pm[warp * 8 + g] = m_run, pl[warp * 8 + g] = l_run;
+        // ---- the unit's end, or the run's
+        const bool done = at.stage + 1 == at.stages;
+        if (done || n + 1 == count) {
+            const bool whole = done && start_stage == 0;
+            float l = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            const int64_t part = 2 * wid + (start == 0 ? 0 : 1);
+            float* dst = whole ? nullptr : sp.scratch + part * sp.heads * HD;
+            T* out = static_cast<T*>(a.out) + (int64_t)at.row * (int64_t)a.out_stride + (int64_t)h0 * HD;
+            if (!whole && t == 0 && g < nh)
+                *reinterpret_cast<float2*>(sp.scratch + ((int64_t)gridDim.x * kWarps * 2 * HD + part * 2) * sp.heads + 2 * g) = make_float2(m_run, l);
+            // sums of the two heads of this lane's columns
+            float inv[2];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = o[b][m][i];
-                if constexpr (PACK) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);  // columns h and h + 4
+            for (int i = 0; i < 2; ++i) {
+                const float x = __shfl_sync(0xffffffffu, l, 8 * t + 4 * i);
+                inv[i] = !whole ? 1.0f : x == 0.0f ? 0.0f : 1.0f / x;
             }
-            if (!PACK || t < 2) {
-                const int d = 32 * b + 4 * g + 2 * m;
-                float* dst = po + (warp * 8 + 2 * t) * HD + d;
-                *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[2]);
-                *reinterpret_cast<float2*>(dst + HD) = make_float2(v[1], v[3]);
-            }
-        }
-    __syncthreads();
-    float* co = pl + kWarps * 8;     // the CTA's result [8][HD], then maxima and sums [8]
-    float* cm = co + 8 * HD;
-    float* cl = cm + 8;
-    for (int i = threadIdx.x; i < nh * HD; i += kWarps * 32) {
-        const int h = i / HD;
-        float mt = -INFINITY, y = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, pm[w * 8 + h]);
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float m = pm[w * 8 + h], c = m == -INFINITY ? 0.0f : ex2(m - mt);
-            y = fmaf(c, po[w * 8 * HD + i], y);
-            l = fmaf(c, pl[w * 8 + h], l);
-        }
-        co[i] = y;
-        if (i % HD == 0) cm[h] = mt, cl[h] = l;
-    }
-    __syncthreads();
-    T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)h0 * HD;
-    if (sp.splits == 1) {
-        for (int i = threadIdx.x; i < nh * HD; i += kWarps * 32) {
-            const float l = cl[i / HD];
-            out[i] = from_f32<T>(l == 0.0f ? 0.0f : co[i] / l);
-        }
-    } else if (sp.scratch) {
-        float* dst = sp.scratch + (int64_t)blockIdx.x * sp.heads * (HD + 2);
-        for (int i = threadIdx.x; i < nh * HD; i += kWarps * 32) dst[i] = co[i];
-        if ((int)threadIdx.x < nh) {
-            dst[sp.heads * HD + threadIdx.x] = cm[threadIdx.x];
-            dst[sp.heads * (HD + 1) + threadIdx.x] = cl[threadIdx.x];
-        }
-    } else {
-        // the cluster's CTAs are this unit's parts: each joins its share of the
-        // elements, reading the others' results from their shared memory
-        cg::cluster_group cl_grp = cg::this_cluster();
-        cl_grp.sync();
-        for (int i = split * (kWarps * 32) + threadIdx.x; i < nh * HD; i += sp.splits * kWarps * 32) {
-            const int h = i / HD;
-            float mt = -INFINITY, y = 0.0f, l = 0.0f;
-            for (int r = 0; r < sp.splits; ++r) mt = fmaxf(mt, cl_grp.map_shared_rank(cm, r)[h]);
-            for (int r = 0; r < sp.splits; ++r) {
-                const float m = cl_grp.map_shared_rank(cm, r)[h], c = m == -INFINITY ? 0.0f : ex2(m - mt);
-                y = fmaf(c, cl_grp.map_shared_rank(co, r)[i], y);
-                l = fmaf(c, cl_grp.map_shared_rank(cl, r)[h], l);
+                for (int m = 0; m < 2; ++m) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = o[b][m][i];
+                        if constexpr (PACK) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);  // columns h and h + 4
+                    }
+                    const int d = 32 * b + 4 * g + 2 * m;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int h = 2 * t + i;
+                        if (h >= nh) continue;
+                        // rows g and g + 8: nibbles 2 m and 2 m + 1
+                        const float y0 = v[i] * (m ? 1.0f / 256 : 1.0f), y1 = v[2 + i] * (m ? 1.0f / 4096 : 1.0f / 16);
+                        if (whole) {
+                            out[h * HD + d] = from_f32<T>(y0 * inv[i]);
+                            out[h * HD + d + 1] = from_f32<T>(y1 * inv[i]);
+                        } else {
+                            *reinterpret_cast<float2*>(dst + h * HD + d) = make_float2(y0, y1);
+                        }
+                    }
+                }
+            if (done && lane == 0 && (sp.by_unit || !whole)) {
+                const int64_t unit = ((int64_t)at.row * H + at.kvh) * sp.chunks + at.chunk;
+                int4 j = make_int4((int)unit, 0, 0, -1);
+                if (!whole) {  // the unit's first stage, and the warp that had it
+                    const int64_t u0 = s0 + start - start_stage, w0 = ((u0 + 1) * W - 1) / total;
+                    j = make_int4((int)unit, (int)(2 * w0 + (w0 * total / W == u0 ? 0 : 1)), (int)w0, (int)wid);
+                }
+                sp.joins[sp.by_unit ? unit : wid] = j;
             }
-            out[i] = from_f32<T>(l == 0.0f ? 0.0f : y / l);
+            fresh = true;
         }
-        cl_grp.sync();  // nobody leaves while another reads its shared memory
+        next(at);
     }
 }
 
-// Joins the parts of one unit's head (a CTA each): out = sum_r 2^(m_r - m) o_r
-// / sum_r 2^(m_r - m) l_r, the parts dealt to groups of HD / 4 threads.
+// Joins the parts of one unit: out = sum_r 2^(m_r - m) o_r / sum_r 2^(m_r - m)
+// l_r, a head at a time (one CTA per head where the units are few).  The parts
+// are dealt to groups of HD / 4 threads, four of a group's parts in flight:
+// with few units it is one long chain of loads from L2 (131,071 tokens, 296
+// parts a unit: 10.7 us with 256 threads and one part in flight).
+constexpr int kJoin = 1024;
 template <class T, int HD>
-__global__ void __launch_bounds__(256) attn_q4_join_kernel(AttnQ4Args a, Q4Split sp) {
-    constexpr int kLane = HD / 4, kGroups = 256 / kLane;
-    __shared__ float c[kMaxSplits], red[kGroups][HD + 1];
-    const int64_t unit = blockIdx.x;
-    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, hs = sp.heads, h = blockIdx.y;
-    const int chunk = (int)(unit % sp.chunks), kvh = (int)(unit / sp.chunks % H);
-    const int64_t row = unit / sp.chunks / H;
-    if (chunk * hs + h >= G) return;
-    const int ctx = (int)max(0, min(a.ctx_len[row], (int)a.max_ctx));
-    const int per = q4_part(ctx, sp.splits, kWarps * Q4Tile<HD>::TT), parts = per ? (ctx + per - 1) / per : 0;
-    const int64_t stride = (int64_t)hs * (HD + 2);
-    const float* src = sp.scratch + unit * sp.splits * stride;
+__global__ void __launch_bounds__(kJoin) attn_q4_join_kernel(AttnQ4Args a, Q4Split sp, int64_t warps) {
+    constexpr int kLane = HD / 4, kGroups = kJoin / kLane;
+    __shared__ float red[kGroups][HD + 1], top[kJoin / 32];
+    const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, hs = sp.heads;
     pdl_wait();
-    float mt = -INFINITY, l = 0.0f;
-    for (int r = threadIdx.x; r < parts; r += 256) mt = fmaxf(mt, src[r * stride + hs * HD + h]);
-    mt = warp_max(mt);
-    if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = mt;
-    __syncthreads();
-    mt = red[0][0];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) mt = fmaxf(mt, red[0][w]);
-    for (int r = threadIdx.x; r < parts; r += 256) {
-        const float m = src[r * stride + hs * HD + h];
-        c[r] = m == -INFINITY ? 0.0f : ex2(m - mt);
+    if (sp.by_unit) {
+        const int64_t row = blockIdx.x / (unsigned)(H * sp.chunks);
+        if (min(a.ctx_len[row], (int)a.max_ctx) <= 0) return;  // nobody wrote the entry
     }
-    __syncthreads();
-    const int d = threadIdx.x % kLane * 4, grp = threadIdx.x / kLane;
-    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int r = grp; r < parts; r += kGroups) {
-        const float w = c[r];
-        const float2 u = *reinterpret_cast<const float2*>(src + r * stride + h * HD + d),
-                     v = *reinterpret_cast<const float2*>(src + r * stride + h * HD + d + 2);
-        y[0] = fmaf(w, u.x, y[0]), y[1] = fmaf(w, u.y, y[1]);
-        y[2] = fmaf(w, v.x, y[2]), y[3] = fmaf(w, v.y, y[3]);
-        if (d == 0) l = fmaf(w, src[r * stride + hs * (HD + 1) + h], l);
-    }
+    const int4 j = sp.joins[blockIdx.x];
+    if (j.w < 0) return;
+    const int chunk = j.x % sp.chunks, kvh = j.x / sp.chunks % H, parts = j.w - j.z + 1;
+    const int64_t row = j.x / sp.chunks / H;
+    const int nh = min(hs, G - chunk * hs);
+    const float* ml = sp.scratch + 2 * warps * HD * hs;
+    auto part = [&](int r) -> int64_t { return r == 0 ? j.y : 2 * (int64_t)(j.z + r); };
+    for (int h = blockIdx.y; h < nh; h += gridDim.y) {
+        float mt = -INFINITY, l = 0.0f;
+        for (int r = threadIdx.x; r < parts; r += blockDim.x) mt = fmaxf(mt, ml[(part(r) * hs + h) * 2]);
+        mt = warp_max(mt);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = mt;
+        __syncthreads();
+        mt = top[0];
+        for (int w = 1; w < (int)blockDim.x / 32; ++w) mt = fmaxf(mt, top[w]);
+        const int d = threadIdx.x % kLane * 4, grp = threadIdx.x / kLane, groups = blockDim.x / kLane;
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = grp; r < parts; r += 4 * groups) {
+            float2 x[4];
+            float4 u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[grp][d + i] = y[i];
-    if (d == 0) red[grp][HD] = l;
-    __syncthreads();
-    T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)(kvh * G + chunk * hs + h) * HD;
-    for (int i = threadIdx.x; i < HD; i += 256) {
-        float v = 0.0f, den = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const int64_t k = part(min(r + i * groups, parts - 1)) * hs + h;
+                x[i] = *reinterpret_cast<const float2*>(ml + k * 2);
+                u[i] = *reinterpret_cast<const float4*>(sp.scratch + k * HD + d);
+            }
 #pragma unroll
-        for (int w = 0; w < kGroups; ++w) v += red[w][i], den += red[w][HD];
-        out[i] = from_f32<T>(den == 0.0f ? 0.0f : v / den);
+            for (int i = 0; i < 4; ++i) {
+                if (r + i * groups >= parts) break;
+                const float c = x[i].x == -INFINITY ? 0.0f : ex2(x[i].x - mt);
+                y[0] = fmaf(c, u[i].x, y[0]), y[1] = fmaf(c, u[i].y, y[1]);
+                y[2] = fmaf(c, u[i].z, y[2]), y[3] = fmaf(c, u[i].w, y[3]);
+                l = fmaf(c, x[i].y, l);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[grp][d + i] = y[i];
+        if (d == 0) red[grp][HD] = l;
+        __syncthreads();
+        T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)(kvh * G + chunk * hs + h) * HD;
+        for (int i = threadIdx.x; i < HD; i += blockDim.x) {
+            float v = 0.0f, den = 0.0f;
+            for (int w = 0; w < groups; ++w) v += red[w][i], den += red[w][HD];
+            out[i] = from_f32<T>(den == 0.0f ? 0.0f : v / den);
+        }
     }
+}
+
+// CTAs of a kernel that the current GPU holds at once.
+uint64_t resident_ctas(const void* kernel, int threads, int smem) {
+    int per = 0, sms = 0, dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem);
+    return (uint64_t)std::max(1, per * sms);
 }
 
 template <class T, int HD, bool PACK>
 cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     using X = Q4Tile<HD>;
-    constexpr int kHeads = PACK ? 4 : 8, kCta = kWarps * X::TT;
-    const int merge = (kWarps * 8 * (HD + 2) + 8 * (HD + 2)) * 4;
-    const int smem = std::max(kWarps * X::kRing + kWarps * kStages * 8, merge);
+    constexpr int kHeads = PACK ? 4 : 8;
+    const int smem = kWarps * X::kRing + kWarps * kStages * 8;
     auto kernel = attn_q4_decode_kernel<T, HD, PACK>;
     ensure_smem_attr(kernel, smem);
-    static const int slots = [&] {  // CTAs that the GPU holds at once
-        int per = 0, sms = 0, dev = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kWarps * 32, smem);
-        return std::max(1, per * sms);
-    }();
+    static const uint64_t slots = resident_ctas(reinterpret_cast<const void*>(kernel), kWarps * 32, smem);
     Q4Split sp{};
     const uint64_t G = a.n_head / a.n_head_kv;
+    sp.heads = (int)std::min<uint64_t>(kHeads, G);
     sp.chunks = (int)((G + kHeads - 1) / kHeads);
     const uint64_t units = a.n_q * a.n_head_kv * sp.chunks;
+    if (units > 0x7fffffffull) return cudaErrorInvalidConfiguration;
     int L = 0;
     while ((1ull << L) < a.page) ++L;
     sp.page_mul = (uint32_t)(((1ull << (31 + L)) + a.page - 1) / a.page);
     sp.page_shift = 31 + L;
-    // enough CTAs to fill the GPU once, none with less than one stage per warp,
-    // and none with more than 2048 tokens (a long sequence among short ones
-    // would otherwise keep one CTA busy after the others are done)
-    const uint64_t stages = (a.max_ctx + kCta - 1) / kCta;
-    uint64_t want = std::max<uint64_t>(slots / units, (a.max_ctx + 2047) / 2048);
-    want = std::max<uint64_t>(1, std::min<uint64_t>({want, stages, kMaxSplits}));
-    sp.heads = (int)std::min<uint64_t>(kHeads, G);
-    if (units * want > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-    if (want > 1 && want <= 8) {  // a cluster
-        int c = 2;
-        while (c < (int)want) c *= 2;
-        sp.splits = c;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(units * c));
-        cfg.blockDim = dim3(kWarps * 32);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)c;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, kernel, a, sp);
-    }
-    sp.splits = (int)want;
-    if (want > 1) keep_pool_memory();
-    if (want > 1)
-        if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&sp.scratch), units * want * sp.heads * (HD + 2) * 4, s))
-            return e;
-    kernel<<<(unsigned)(units * want), kWarps * 32, smem, s>>>(a, sp);
+    const uint64_t most = units * ((a.max_ctx + X::TT - 1) / X::TT);  // stages
+    if (most > (1ull << 40)) return cudaErrorInvalidConfiguration;  // a warp counts its stages in 32 bits
+    const uint64_t grid = std::max<uint64_t>(1, std::min<uint64_t>(slots, most)), warps = grid * kWarps;
+    sp.by_unit = units <= warps;
+    const uint64_t joins = sp.by_unit ? units : warps;
+    keep_pool_memory();
+    const uint64_t parts = 2 * warps * sp.heads * (HD + 2) * 4;
+    uint8_t* scratch = nullptr;
+    if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), parts + joins * sizeof(int4), s)) return e;
+    sp.scratch = reinterpret_cast<float*>(scratch);
+    sp.joins = reinterpret_cast<int4*>(scratch + parts);
+    // many parts a unit: all 1024 threads; few: as many groups as there are parts, at most
+    const uint64_t unit_parts = std::min(warps, most) / std::max<uint64_t>(1, std::min(units, warps)) + 2;
+    const unsigned join_threads = (unsigned)std::min<uint64_t>(kJoin, std::max<uint64_t>(128, (unit_parts * (HD / 4) + 127) / 128 * 128));
+    const dim3 join_grid((unsigned)joins, sp.by_unit ? (unsigned)sp.heads : 1u, 1u);
+    kernel<<<(unsigned)grid, kWarps * 32, smem, s>>>(a, sp);
     cudaError_t e = cudaGetLastError();
-    if (want > 1) {
-        if (e == cudaSuccess) {
-            e = launch_pdl(attn_q4_join_kernel<T, HD>, dim3((unsigned)units, (unsigned)sp.heads), dim3(256), 0, s, a, sp);
-        }
-        cudaFreeAsync(sp.scratch, s);
-    }
+    if (e == cudaSuccess)
+        e = launch_pdl(attn_q4_join_kernel<T, HD>, join_grid, dim3(join_threads), 0, s, a, sp, (int64_t)warps);
+    cudaFreeAsync(scratch, s);
     return e;
 }
 template <class T>
