@@ -235,7 +235,7 @@ struct Q4Split {
     int by_unit;
     int heads;         // query heads of a unit at most
     int chunks;        // units per kv head
-    uint32_t page_mul; // t / page = t * page_mul >> page_shift for t < 2^31
+    uint32_t page_mul; // t / page = (2 t page_mul >> 32) >> page_shift for t < 2^31
     int page_shift;
 };
 
@@ -250,7 +250,6 @@ __device__ __forceinline__ int q4_stages(const AttnQ4Args& a, int64_t row) {
 struct Q4Place {
     int row, kvh, chunk;
     int stage, stages;  // of this unit
-    int ctx;
 };
 
 // words b = 0 .. NB - 1 at 32-bit word t * NB + b of a swizzled row
@@ -305,14 +304,14 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     pdl_trigger();  // the join may be set up as soon as there is room
     // ---- this warp's run of stages.  Thread i sums the stages of rows i R ..
     // i R + R - 1; the warp finds the thread, then the row, where its run starts.
-    const int64_t n_row = (int64_t)a.n_q, R = (n_row + kWarps * 32 - 1) / (kWarps * 32);
-    int64_t* before = reinterpret_cast<int64_t*>(smem);  // [129], in the ring's place
-    int64_t mine = 0;
-    for (int64_t r = threadIdx.x * R; r < min(n_row, (threadIdx.x + 1) * R); ++r) mine += q4_stages<HD>(a, r);
-    int64_t upto = mine;
+    // (The host sees to it that all of this fits 32 bits.)
+    const int n_row = (int)a.n_q, R = (n_row + kWarps * 32 - 1) / (kWarps * 32);
+    int* before = reinterpret_cast<int*>(smem);  // [129 + 4], in the ring's place
+    int upto = 0;
+    for (int i = 0, r = threadIdx.x * R; i < R && r < n_row; ++i, ++r) upto += q4_stages<HD>(a, r);
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, k);
+        const int x = __shfl_up_sync(0xffffffffu, upto, k);
         if (lane >= k) upto += x;
     }
     if (lane == 31) before[kWarps * 32 + 1 + warp] = upto;
@@ -321,39 +320,44 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     before[threadIdx.x + 1] = upto;
     if (threadIdx.x == 0) before[0] = 0;
     __syncthreads();
-    const int64_t total = before[kWarps * 32] * upr;
-    // warp numbers run over the CTAs first, so that few stages spread over all SMs
-    const int64_t W = min((int64_t)gridDim.x * kWarps, total), wid = (int64_t)warp * gridDim.x + blockIdx.x;
-    const int64_t s0 = wid < W ? wid * total / W : 0, s1 = wid < W ? (wid + 1) * total / W : 0;
-    Q4Place at{0, 0, 0, 0, 1, 0};
-    if (s0 < s1) {
+    const uint32_t total = (uint32_t)before[kWarps * 32] * (uint32_t)upr;
+    // `longer` warps take base + 1 stages, the others base.  Warp numbers run
+    // over the CTAs first, so that few stages spread over all SMs.
+    const uint32_t W = min(gridDim.x * kWarps, total), wid = (uint32_t)warp * gridDim.x + blockIdx.x;
+    const uint32_t base = W ? total / W : 0, longer = total - base * W;
+    const uint32_t s0 = wid * base + min(wid, longer);
+    const int count = wid < W ? (int)(base + (wid < longer)) : 0;
+    Q4Place at{0, 0, 0, 0, 1};
+    if (count) {
         int n = 0;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) n += __popc(__ballot_sync(0xffffffffu, before[k * 32 + lane] * upr <= s0));
-        int64_t rest = s0 - before[n - 1] * upr;
-        at.row = (int)((n - 1) * R);
+        for (int k = 0; k < kWarps; ++k)
+            n += __popc(__ballot_sync(0xffffffffu, (uint32_t)before[k * 32 + lane] * (uint32_t)upr <= s0));
+        uint32_t rest = s0 - (uint32_t)before[n - 1] * (uint32_t)upr;
+        at.row = (n - 1) * R;
         while (true) {
             at.stages = q4_stages<HD>(a, at.row);
-            if (rest < (int64_t)at.stages * upr) break;
-            rest -= (int64_t)at.stages * upr;
+            if (rest < (uint32_t)at.stages * (uint32_t)upr) break;
+            rest -= (uint32_t)at.stages * (uint32_t)upr;
             ++at.row;
         }
-        const int u = (int)(rest / at.stages);
-        at.stage = (int)(rest - (int64_t)u * at.stages);
-        at.kvh = u / sp.chunks;
-        at.chunk = u % sp.chunks;
-        at.ctx = min(a.ctx_len[at.row], (int)a.max_ctx);
+        const uint32_t u = rest / (uint32_t)at.stages;
+        at.stage = (int)(rest - u * (uint32_t)at.stages);
+        at.kvh = (int)(u / (uint32_t)sp.chunks);
+        at.chunk = (int)(u % (uint32_t)sp.chunks);
     }
     __syncthreads();  // `before` has been read
-    // rows with no tokens give zeros
-    for (int64_t r = blockIdx.x; r < n_row; r += gridDim.x)
-        if (min(a.ctx_len[r], (int)a.max_ctx) <= 0)
+    // rows with no tokens give zeros, and nothing to join
+    for (int r = blockIdx.x; r < n_row; r += gridDim.x)
+        if (min(a.ctx_len[r], (int)a.max_ctx) <= 0) {
             for (int i = threadIdx.x; i < (int)a.n_head * HD; i += kWarps * 32)
                 static_cast<T*>(a.out)[r * (int64_t)a.out_stride + i] = from_f32<T>(0.0f);
-    if (!sp.by_unit && lane == 0) sp.joins[(int64_t)warp * gridDim.x + blockIdx.x].w = -1;
-    if (s0 >= s1) return;
-    auto next = [&](Q4Place& p) {
-        if (++p.stage < p.stages) return;
+            for (int i = threadIdx.x; sp.by_unit && i < upr; i += kWarps * 32)
+                sp.joins[(int64_t)r * upr + i].w = -1;
+        }
+    if (!sp.by_unit && lane == 0) sp.joins[wid].w = -1;
+    if (!count) return;
+    auto next_unit = [&](Q4Place& p) {
         p.stage = 0;
         if (++p.chunk < sp.chunks) return;
         p.chunk = 0;
@@ -363,28 +367,37 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
             if (++p.row >= n_row) return;
             p.stages = q4_stages<HD>(a, p.row);
         } while (p.stages == 0);
-        p.ctx = min(a.ctx_len[p.row], (int)a.max_ctx);
     };
 
     uint8_t* ring = smem + warp * X::kRing;
-    const uint32_t ring_s = smem_u32(ring);
-    uint32_t* valid_ring = reinterpret_cast<uint32_t*>(smem + kWarps * X::kRing) + warp * kStages * 2;
 
     // ---- copies.  Lane l looks the cache slots of tokens l (and l + 32) of a
-    // stage up; `exists` has a bit for each that is there.
+    // stage up, one stage ahead of its copies; `exists` has a bit for each that
+    // is there.
     constexpr int LT = TT > 32 ? TT / 32 : 1;
     uint32_t slots[LT], exists;
-    auto look_up = [&](const Q4Place& p) {
+    Q4Place ahead = at;
+    int left = count;       // stages to copy
+    const int32_t* table;   // of the sequence being copied
+    int ctx;
+    uint32_t head_slot;
+    const uint32_t page = (uint32_t)a.page, page_rows = (uint32_t)H * page;
+    auto new_unit = [&] {
+        table = a.block_table + (int64_t)ahead.row * (int64_t)a.max_pages;
+        ctx = min(a.ctx_len[ahead.row], (int)a.max_ctx);
+        head_slot = (uint32_t)ahead.kvh * page;
+    };
+    auto look_up = [&] {
         exists = 0;
 #pragma unroll
         for (int i = 0; i < LT; ++i) {
-            const uint32_t tok = (uint32_t)p.stage * TT + lane + 32 * i;
+            const uint32_t tok = (uint32_t)ahead.stage * TT + lane + 32 * i;
             slots[i] = 0;
-            if (tok < (uint32_t)p.ctx && (TT >= 32 || lane < TT)) {
-                const uint32_t pi = (uint32_t)(((uint64_t)tok * sp.page_mul) >> sp.page_shift);
-                const uint32_t pg = (uint32_t)a.block_table[(int64_t)p.row * (int64_t)a.max_pages + pi];
+            if (tok < (uint32_t)ctx && (TT >= 32 || lane < TT)) {
+                const uint32_t pi = __umulhi(tok << 1, sp.page_mul) >> sp.page_shift;
+                const uint32_t pg = (uint32_t)table[pi];
                 if (pg < (uint32_t)a.n_pages) {
-                    slots[i] = (pg * (uint32_t)H + (uint32_t)p.kvh) * (uint32_t)a.page + (tok - pi * (uint32_t)a.page);
+                    slots[i] = pg * page_rows + (head_slot + tok - pi * page);
                     exists |= 1u << i;
                 }
             }
@@ -394,8 +407,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     // its score -inf -- so only the scale copies carry a size
     const uint8_t* k_unit = a.k_pages + lane % X::U * 16;
     const uint8_t* v_unit = a.v_pages + lane % X::U * 16;
-    auto issue = [&](int s) {
-        const uint32_t st = ring_s + s * X::kBytes;
+    uint32_t valid[kStages][LT];  // tokens that are there: [0] of the stage computed next
+    auto issue = [&](uint32_t st, int k) {
 #pragma unroll
         for (int i = 0; i < 2048 / 16 / 32; ++i) {
             const int r = (i * 32 + lane) / X::U;  // unit lane % U of token r
@@ -413,18 +426,20 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
                 cp_async_fill<NB * 2>(dst, a.k_scales + off, ok ? NB * 2 : 0);
                 cp_async_fill<NB * 2>(dst + X::kScale, a.v_scales + off, ok ? NB * 2 : 0);
             }
-            const uint32_t v = __ballot_sync(0xffffffffu, ok);
-            if (lane == 0) valid_ring[s * 2 + i] = v;
+            valid[k][i] = __ballot_sync(0xffffffffu, ok);
         }
     };
-    Q4Place ahead = at;
-    int left = (int)(s1 - s0);  // stages to copy
-    look_up(ahead);
+    const uint32_t ring_s = smem_u32(ring);
+    new_unit();
+    look_up();
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
+    for (int k = 0; k < kStages - 1; ++k) {
         if (left > 0) {
-            issue(s);
-            if (--left) next(ahead), look_up(ahead);
+            issue(ring_s + k * X::kBytes, k);
+            if (--left) {
+                if (++ahead.stage == ahead.stages) next_unit(ahead), new_unit();
+                look_up();
+            }
         }
         cp_async_commit();
     }
@@ -435,281 +450,272 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     const int hrow = PACK ? (g & 3) : g;
     uint32_t qa[NB][2][kTwo ? 4 : 2];
     float c_h;
-    int h0, nh;
 
     const uint64_t bias0 = held_pair(-8388616.0f, -8388736.0f), bias1 = held_pair(-8390656.0f, -8421376.0f);
     const uint32_t first = g >= 4 ? 0xffffe000u : 0u;
     float o[NB][2][4];  // [block][dims 4g + 2 mu + {0, 1}][heads 2t, 2t + 1 of rows g, g + 8]
     float m_run = -INFINITY, l_run = 0.0f;
-    const int count = (int)(s1 - s0);
-    int start = 0, start_stage = at.stage;  // where this warp's part of the unit begins, and its stage there
-    bool fresh = true;
-    int s = 0;
-    for (int n = 0; n < count; ++n) {
-        if (fresh) {
-            h0 = at.kvh * G + at.chunk * sp.heads;
-            nh = min(sp.heads, G - at.chunk * sp.heads);
-            const T* q = static_cast<const T*>(a.q) + (int64_t)at.row * (int64_t)a.q_stride + (int64_t)(h0 + min(hrow, nh - 1)) * HD;
-            float x[NB][8], mx = 0.0f;
+    uint32_t off = 0, refill = (kStages - 1) * X::kBytes;  // of the stage computed, and of the one copied into
+    for (int n = 0; n < count;) {
+        // this warp's part of the unit: stages at.stage .. end - 1
+        const int from = at.stage, end = min(at.stages, from + count - n), start = n;
+        const int h0 = at.kvh * G + at.chunk * sp.heads, nh = min(sp.heads, G - at.chunk * sp.heads);
+        const T* q = static_cast<const T*>(a.q) + (int64_t)at.row * (int64_t)a.q_stride + (int64_t)(h0 + min(hrow, nh - 1)) * HD;
+        float x[NB][8], mx = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                load_n<8, true>(q + 32 * b + 8 * t, x[b]);
+        for (int b = 0; b < NB; ++b) {
+            load_n<8, true>(q + 32 * b + 8 * t, x[b]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[b][i]));
-            }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // times 2^e: the largest below 2^15
-            const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
-            const float up = pow2i(e);
-            c_h = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[b][i] *= up;
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const float f[4] = {x[b][2 * s], x[b][2 * s + 4], x[b][2 * s + 1] * 0.0625f,
-                                        x[b][2 * s + 5] * 0.0625f};
-                    float lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) lo[i] = f[i] - __half2float(__float2half_rn(f[i]));
-                    if constexpr (kTwo) {
-                        qa[b][s][0] = pack_half2(f[0], f[1]);
-                        qa[b][s][1] = pack_half2(lo[0], lo[1]);
-                        qa[b][s][2] = pack_half2(f[2], f[3]);
-                        qa[b][s][3] = pack_half2(lo[2], lo[3]);
-                    } else {
-                        qa[b][s][0] = pack_half2(f[0], f[1]);
-                        qa[b][s][1] = pack_half2(f[2], f[3]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
-            m_run = -INFINITY;
-            l_run = 0.0f;
-            start = n;
-            start_stage = at.stage;
-            fresh = false;
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[b][i]));
         }
-        cp_async_wait<kStages - 2>();
-        __syncwarp();
-        const uint8_t* kt = ring + s * X::kBytes;
-        const uint8_t* vt = kt + 2048;
-        const uint8_t* ksc = kt + 4096;
-        const uint8_t* vsc = ksc + X::kScale;
-
-        // ---- scores
-        float sc[NJ][2];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            uint32_t w[NB], d[NB];
-            load_words<HD>(w, kt, 8 * j + g, t);
-            load_scales<HD>(d, ksc, 8 * j + 2 * t);
-            uint64_t sum = 0;  // two zeros
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t x = k ? w[b] >> 8 : w[b];
-                    uint32_t qf[4];
-                    if constexpr (kTwo) {
-                        qf[0] = qa[b][k][0], qf[1] = qa[b][k][1], qf[2] = qa[b][k][2], qf[3] = qa[b][k][3];
-                    } else {
-                        qf[0] = qa[b][k][0], qf[1] = 0, qf[2] = qa[b][k][1], qf[3] = 0;
-                    }
-                    mma16816(c, qf, nib_lo(x), nib_hi(x), c);
-                }
-                const uint64_t dd = pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b));
-                uint64_t cc = pair(c[0], c[1]);
-                if constexpr (kTwo) cc = f2_add(cc, pair(c[2], c[3]));
-                sum = tc::f2_fma(cc, dd, sum);
-            }
-            unpair(sum, sc[j][0], sc[j][1]);
-        }
-        // tokens that do not exist
-#pragma unroll
-        for (int i = 0; i < LT; ++i) {
-            const uint32_t v = valid_ring[s * 2 + i], full = TT >= 32 ? 0xffffffffu : (1u << (TT & 31)) - 1u;
-            if (v != full) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (j / 4 == i) {
-                        const uint32_t k = v >> (8 * (j % 4) + 2 * t);
-                        if (!(k & 1u)) sc[j][0] = -INFINITY;
-                        if (!(k & 2u)) sc[j][1] = -INFINITY;
-                    }
-            }
-        }
-        // ---- running maximum, weights
-        float mx = sc[0][0];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(sc[j][0], sc[j][1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run, mx * c_h), m_use = m_new == -INFINITY ? 0.0f : m_new;
-        if (__any_sync(0xffffffffu, m_new != m_run)) {
-            const float alpha = m_run == -INFINITY ? 0.0f : ex2(m_run - m_use);
-            l_run *= alpha;
-            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+        // times 2^e: the largest below 2^15
+        const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+        const float up = pow2i(e);
+        c_h = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    o[b][m][0] *= a0, o[b][m][1] *= a1;
-                    o[b][m][2] *= a0, o[b][m][3] *= a1;
+            for (int i = 0; i < 8; ++i) x[b][i] *= up;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const float f[4] = {x[b][2 * s], x[b][2 * s + 4], x[b][2 * s + 1] * 0.0625f,
+                                    x[b][2 * s + 5] * 0.0625f};
+                float lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lo[i] = f[i] - __half2float(__float2half_rn(f[i]));
+                if constexpr (kTwo) {
+                    qa[b][s][0] = pack_half2(f[0], f[1]);
+                    qa[b][s][1] = pack_half2(lo[0], lo[1]);
+                    qa[b][s][2] = pack_half2(f[2], f[3]);
+                    qa[b][s][3] = pack_half2(lo[2], lo[3]);
+                } else {
+                    qa[b][s][0] = pack_half2(f[0], f[1]);
+                    qa[b][s][1] = pack_half2(f[2], f[3]);
                 }
-            m_run = m_new;
-        }
-        // ---- outputs, 8 tokens at a time
-        const int half = (g & 1) * 16;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            float p[2];
-            uint32_t d[NB], w[2][NB];
-            load_scales<HD>(d, vsc, 8 * j + 2 * t);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
-                l_run += p[i];
-                if constexpr (!kTwo) p[i] *= 1.000244140625f;
-                load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
             }
-            const uint64_t pp = pair(p[0], p[1]);
+        }
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float v[2];
-                const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
-                unpair(vv, v[0], v[1]);
-                const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
-                float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
-                values2<0>(x0, bias0, f0[0], f0[1]);
-                values2<0>(x1, bias0, f0[2], f0[3]);
-                values2<2>(x0, bias1, f1[0], f1[1]);
-                values2<2>(x1, bias1, f1[2], f1[3]);
-                if constexpr (PACK) {
-                    // columns 0..3: v, cut to 11 bits by the MMA; 4..7: v less its first 11 bits
-                    const uint64_t cut = pair(-__uint_as_float(__float_as_uint(v[0]) & first),
-                                              -__uint_as_float(__float_as_uint(v[1]) & first));
-                    unpair(f2_add(vv, cut), v[0], v[1]);
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
+        m_run = -INFINITY;
+        l_run = 0.0f;
+        for (; at.stage < end; ++at.stage, ++n) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
+            const uint8_t* kt = ring + off;
+            const uint8_t* vt = kt + 2048;
+            const uint8_t* ksc = kt + 4096;
+            const uint8_t* vsc = ksc + X::kScale;
+
+            // ---- scores
+            float sc[NJ][2];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                uint32_t w[NB], d[NB];
+                load_words<HD>(w, kt, 8 * j + g, t);
+                load_scales<HD>(d, ksc, 8 * j + 2 * t);
+                uint64_t sum = 0;  // two zeros
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t x = k ? w[b] >> 8 : w[b];
+                        uint32_t qf[4];
+                        if constexpr (kTwo) {
+                            qf[0] = qa[b][k][0], qf[1] = qa[b][k][1], qf[2] = qa[b][k][2], qf[3] = qa[b][k][3];
+                        } else {
+                            qf[0] = qa[b][k][0], qf[1] = 0, qf[2] = qa[b][k][1], qf[3] = 0;
+                        }
+                        mma16816(c, qf, nib_lo(x), nib_hi(x), c);
+                    }
+                    const uint64_t dd = pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b));
+                    uint64_t cc = pair(c[0], c[1]);
+                    if constexpr (kTwo) cc = f2_add(cc, pair(c[2], c[3]));
+                    sum = tc::f2_fma(cc, dd, sum);
                 }
-                mma1688(o[b][0], f0, v[0], v[1]);
-                mma1688(o[b][1], f1, v[0], v[1]);
-                if constexpr (kTwo && !PACK) {
+                unpair(sum, sc[j][0], sc[j][1]);
+            }
+            // tokens that do not exist
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
+            for (int i = 0; i < LT; ++i) {
+                const uint32_t v = valid[0][i], full = TT >= 32 ? 0xffffffffu : (1u << (TT & 31)) - 1u;
+                if (v != full) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        if (j / 4 == i) {
+                            const uint32_t k = v >> (8 * (j % 4) + 2 * t);
+                            if (!(k & 1u)) sc[j][0] = -INFINITY;
+                            if (!(k & 2u)) sc[j][1] = -INFINITY;
+                        }
+                }
+            }
+            // ---- running maximum, weights
+            float mx = sc[0][0];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(sc[j][0], sc[j][1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // The reference m follows the maximum only once that is 2^8 above it:
+            // weights up to 2^8 do no harm, and the outputs are seldom rescaled.
+            mx *= c_h;
+            if (__any_sync(0xffffffffu, mx > m_run + 8.0f)) {
+                const float m_new = fmaxf(m_run, mx), alpha = m_new == -INFINITY ? 0.0f : ex2(m_run - m_new);
+                l_run *= alpha;
+                const uint64_t aa = pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2)
+                            unpair(tc::f2_mul(pair(o[b][m][i], o[b][m][i + 1]), aa), o[b][m][i], o[b][m][i + 1]);
+                m_run = m_new;
+            }
+            const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+            // ---- outputs, 8 tokens at a time
+            const int half = (g & 1) * 16;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                float p[2];
+                uint32_t d[NB], w[2][NB];
+                load_scales<HD>(d, vsc, 8 * j + 2 * t);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
+                    l_run += p[i];
+                    if constexpr (!kTwo) p[i] *= 1.000244140625f;
+                    load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
+                }
+                const uint64_t pp = pair(p[0], p[1]);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float v[2];
+                    const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
+                    unpair(vv, v[0], v[1]);
+                    const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
+                    float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
+                    values2<0>(x0, bias0, f0[0], f0[1]);
+                    values2<0>(x1, bias0, f0[2], f0[3]);
+                    values2<2>(x0, bias1, f1[0], f1[1]);
+                    values2<2>(x1, bias1, f1[2], f1[3]);
+                    if constexpr (PACK) {
+                        // columns 0..3: v, cut to 11 bits by the MMA; 4..7: v less its first 11 bits
+                        const uint64_t cut = pair(-__uint_as_float(__float_as_uint(v[0]) & first),
+                                                  -__uint_as_float(__float_as_uint(v[1]) & first));
+                        unpair(f2_add(vv, cut), v[0], v[1]);
+                    }
                     mma1688(o[b][0], f0, v[0], v[1]);
                     mma1688(o[b][1], f1, v[0], v[1]);
+                    if constexpr (kTwo && !PACK) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
+                        mma1688(o[b][0], f0, v[0], v[1]);
+                        mma1688(o[b][1], f1, v[0], v[1]);
+                    }
                 }
             }
+            // ---- the next copies, into the stage used before this one
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k + 1 < kStages; ++k)
+#pragma unroll
+                for (int i = 0; i < LT; ++i) valid[k][i] = valid[k + 1][i];
+            if (left > 0) {
+                issue(ring_s + refill, kStages - 2);
+                if (--left) {
+                    if (++ahead.stage == ahead.stages) next_unit(ahead), new_unit();
+                    look_up();
+                }
+            }
+            cp_async_commit();
+            refill = off;
+            off = off + X::kBytes == X::kRing ? 0 : off + X::kBytes;
         }
-        // ---- the next copies, into the stage used before this one
-        __syncwarp();
-        if (left > 0) {
-            issue((s + kStages - 1) % kStages);
-            if (--left) next(ahead), look_up(ahead);
-        }
-        cp_async_commit();
-        s = s + 1 == kStages ? 0 : s + 1;
 
         // ---- the unit's end, or the run's
-        const bool done = at.stage + 1 == at.stages;
-        if (done || n + 1 == count) {
-            const bool whole = done && start_stage == 0;
-            float l = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            const int64_t part = 2 * wid + (start == 0 ? 0 : 1);
-            float* dst = whole ? nullptr : sp.scratch + part * sp.heads * HD;
-            T* out = static_cast<T*>(a.out) + (int64_t)at.row * (int64_t)a.out_stride + (int64_t)h0 * HD;
-            if (!whole && t == 0 && g < nh)
-                *reinterpret_cast<float2*>(sp.scratch + ((int64_t)gridDim.x * kWarps * 2 * HD + part * 2) * sp.heads + 2 * g) = make_float2(m_run, l);
-            // sums of the two heads of this lane's columns
-            float inv[2];
+        const bool done = at.stage == at.stages;
+        const bool whole = done && from == 0;
+        float l = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        const int64_t part = 2 * (int64_t)wid + (start == 0 ? 0 : 1);
+        float* dst = whole ? nullptr : sp.scratch + part * sp.heads * HD;
+        T* out = static_cast<T*>(a.out) + (int64_t)at.row * (int64_t)a.out_stride + (int64_t)h0 * HD;
+        if (!whole && t == 0 && g < nh)
+            *reinterpret_cast<float2*>(sp.scratch + ((int64_t)gridDim.x * kWarps * 2 * HD + part * 2) * sp.heads + 2 * g) = make_float2(m_run, l);
+        // sums of the two heads of this lane's columns
+        float inv[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float x = __shfl_sync(0xffffffffu, l, 8 * t + 4 * i);
-                inv[i] = !whole ? 1.0f : x == 0.0f ? 0.0f : 1.0f / x;
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[i] = o[b][m][i];
-                        if constexpr (PACK) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);  // columns h and h + 4
-                    }
-                    const int d = 32 * b + 4 * g + 2 * m;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int h = 2 * t + i;
-                        if (h >= nh) continue;
-                        // rows g and g + 8: nibbles 2 m and 2 m + 1
-                        const float y0 = v[i] * (m ? 1.0f / 256 : 1.0f), y1 = v[2 + i] * (m ? 1.0f / 4096 : 1.0f / 16);
-                        if (whole) {
-                            out[h * HD + d] = from_f32<T>(y0 * inv[i]);
-                            out[h * HD + d + 1] = from_f32<T>(y1 * inv[i]);
-                        } else {
-                            *reinterpret_cast<float2*>(dst + h * HD + d) = make_float2(y0, y1);
-                        }
-                    }
-                }
-            if (done && lane == 0 && (sp.by_unit || !whole)) {
-                const int64_t unit = ((int64_t)at.row * H + at.kvh) * sp.chunks + at.chunk;
-                int4 j = make_int4((int)unit, 0, 0, -1);
-                if (!whole) {  // the unit's first stage, and the warp that had it
-                    const int64_t u0 = s0 + start - start_stage, w0 = ((u0 + 1) * W - 1) / total;
-                    j = make_int4((int)unit, (int)(2 * w0 + (w0 * total / W == u0 ? 0 : 1)), (int)w0, (int)wid);
-                }
-                sp.joins[sp.by_unit ? unit : wid] = j;
-            }
-            fresh = true;
+        for (int i = 0; i < 2; ++i) {
+            const float x = __shfl_sync(0xffffffffu, l, 8 * t + 4 * i);
+            inv[i] = !whole ? 1.0f : x == 0.0f ? 0.0f : 1.0f / x;
         }
-        next(at);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = o[b][m][i];
+                    if constexpr (PACK) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);  // columns h and h + 4
+                }
+                const int d = 32 * b + 4 * g + 2 * m;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int h = 2 * t + i;
+                    if (h >= nh) continue;
+                    // rows g and g + 8: nibbles 2 m and 2 m + 1
+                    const float y0 = v[i] * (m ? 1.0f / 256 : 1.0f), y1 = v[2 + i] * (m ? 1.0f / 4096 : 1.0f / 16);
+                    if (whole) {
+                        out[h * HD + d] = from_f32<T>(y0 * inv[i]);
+                        out[h * HD + d + 1] = from_f32<T>(y1 * inv[i]);
+                    } else {
+                        *reinterpret_cast<float2*>(dst + h * HD + d) = make_float2(y0, y1);
+                    }
+                }
+            }
+        if (done && lane == 0 && (sp.by_unit || !whole)) {
+            const int64_t unit = ((int64_t)at.row * H + at.kvh) * sp.chunks + at.chunk;
+            int4 j = make_int4((int)unit, 0, 0, -1);
+            if (!whole) {  // the unit's first stage, and the warp that had it
+                const uint32_t u0 = s0 + (uint32_t)start - (uint32_t)from, edge = longer * (base + 1);
+                const uint32_t w0 = u0 < edge ? u0 / (base + 1) : longer + (u0 - edge) / base;
+                const bool at_start = u0 == w0 * base + min(w0, longer);
+                j = make_int4((int)unit, (int)(2 * w0 + (at_start ? 0 : 1)), (int)w0, (int)wid);
+            }
+            sp.joins[sp.by_unit ? unit : wid] = j;
+        }
+        if (done) next_unit(at);
     }
 }
 
 // Joins the parts of one unit: out = sum_r 2^(m_r - m) o_r / sum_r 2^(m_r - m)
 // l_r, a head at a time (one CTA per head where the units are few).  The parts
-// are dealt to groups of HD / 4 threads, four of a group's parts in flight:
-// with few units it is one long chain of loads from L2 (131,071 tokens, 296
-// parts a unit: 10.7 us with 256 threads and one part in flight).
+// are dealt to groups of HD / 4 threads, four of a group's parts in flight,
+// each group with a maximum of its own; the groups are joined in shared memory.
 constexpr int kJoin = 1024;
 template <class T, int HD>
 __global__ void __launch_bounds__(kJoin) attn_q4_join_kernel(AttnQ4Args a, Q4Split sp, int64_t warps) {
     constexpr int kLane = HD / 4, kGroups = kJoin / kLane;
-    __shared__ float red[kGroups][HD + 1], top[kJoin / 32];
+    __shared__ float red[kGroups][HD + 2];
     const int G = (int)(a.n_head / a.n_head_kv), H = (int)a.n_head_kv, hs = sp.heads;
     pdl_wait();
-    if (sp.by_unit) {
-        const int64_t row = blockIdx.x / (unsigned)(H * sp.chunks);
-        if (min(a.ctx_len[row], (int)a.max_ctx) <= 0) return;  // nobody wrote the entry
-    }
     const int4 j = sp.joins[blockIdx.x];
     if (j.w < 0) return;
     const int chunk = j.x % sp.chunks, kvh = j.x / sp.chunks % H, parts = j.w - j.z + 1;
     const int64_t row = j.x / sp.chunks / H;
     const int nh = min(hs, G - chunk * hs);
     const float* ml = sp.scratch + 2 * warps * HD * hs;
+    const int d = threadIdx.x % kLane * 4, grp = threadIdx.x / kLane, groups = blockDim.x / kLane;
     auto part = [&](int r) -> int64_t { return r == 0 ? j.y : 2 * (int64_t)(j.z + r); };
     for (int h = blockIdx.y; h < nh; h += gridDim.y) {
-        float mt = -INFINITY, l = 0.0f;
-        for (int r = threadIdx.x; r < parts; r += blockDim.x) mt = fmaxf(mt, ml[(part(r) * hs + h) * 2]);
-        mt = warp_max(mt);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = mt;
-        __syncthreads();
-        mt = top[0];
-        for (int w = 1; w < (int)blockDim.x / 32; ++w) mt = fmaxf(mt, top[w]);
-        const int d = threadIdx.x % kLane * 4, grp = threadIdx.x / kLane, groups = blockDim.x / kLane;
-        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = -INFINITY, l = 0.0f;
         for (int r = grp; r < parts; r += 4 * groups) {
             float2 x[4];
             float4 u[4];
@@ -721,21 +727,27 @@ __global__ void __launch_bounds__(kJoin) attn_q4_join_kernel(AttnQ4Args a, Q4Spl
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (r + i * groups >= parts) break;
-                const float c = x[i].x == -INFINITY ? 0.0f : ex2(x[i].x - mt);
-                y[0] = fmaf(c, u[i].x, y[0]), y[1] = fmaf(c, u[i].y, y[1]);
-                y[2] = fmaf(c, u[i].z, y[2]), y[3] = fmaf(c, u[i].w, y[3]);
-                l = fmaf(c, x[i].y, l);
+                if (r + i * groups >= parts || x[i].x == -INFINITY) continue;
+                const float m = fmaxf(top, x[i].x), e = ex2(top - m), c = ex2(x[i].x - m);
+                y[0] = fmaf(c, u[i].x, e * y[0]), y[1] = fmaf(c, u[i].y, e * y[1]);
+                y[2] = fmaf(c, u[i].z, e * y[2]), y[3] = fmaf(c, u[i].w, e * y[3]);
+                l = fmaf(c, x[i].y, e * l);
+                top = m;
             }
         }
+        __syncthreads();  // the last head's sums have been read
 #pragma unroll
         for (int i = 0; i < 4; ++i) red[grp][d + i] = y[i];
-        if (d == 0) red[grp][HD] = l;
+        if (d == 0) red[grp][HD] = l, red[grp][HD + 1] = top;
         __syncthreads();
         T* out = static_cast<T*>(a.out) + row * (int64_t)a.out_stride + (int64_t)(kvh * G + chunk * hs + h) * HD;
         for (int i = threadIdx.x; i < HD; i += blockDim.x) {
-            float v = 0.0f, den = 0.0f;
-            for (int w = 0; w < groups; ++w) v += red[w][i], den += red[w][HD];
+            float v = 0.0f, den = 0.0f, m = -INFINITY;
+            for (int w = 0; w < groups; ++w) m = fmaxf(m, red[w][HD + 1]);
+            for (int w = 0; w < groups; ++w) {
+                const float c = red[w][HD + 1] == -INFINITY ? 0.0f : ex2(red[w][HD + 1] - m);
+                v = fmaf(c, red[w][i], v), den = fmaf(c, red[w][HD], den);
+            }
             out[i] = from_f32<T>(den == 0.0f ? 0.0f : v / den);
         }
     }
@@ -767,9 +779,9 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     int L = 0;
     while ((1ull << L) < a.page) ++L;
     sp.page_mul = (uint32_t)(((1ull << (31 + L)) + a.page - 1) / a.page);
-    sp.page_shift = 31 + L;
+    sp.page_shift = L;
     const uint64_t most = units * ((a.max_ctx + X::TT - 1) / X::TT);  // stages
-    if (most > (1ull << 40)) return cudaErrorInvalidConfiguration;  // a warp counts its stages in 32 bits
+    if (most >= (1ull << 31) || a.n_q > 0x7fffff00ull) return cudaErrorInvalidConfiguration;  // counted in 32 bits
     const uint64_t grid = std::max<uint64_t>(1, std::min<uint64_t>(slots, most)), warps = grid * kWarps;
     sp.by_unit = units <= warps;
     const uint64_t joins = sp.by_unit ? units : warps;
