@@ -122,17 +122,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return reinterpret_cast<const uint32_t&>(h);
-}
-// 2^e for -126 <= e <= 127
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // D (16 x 8, fp32) += A (16 x 8, tf32) B (8 x 8, tf32)
 __device__ __forceinline__ void mma1688(float (&d)[4], const float (&a)[4], float b0, float b1) {
     asm volatile(
@@ -141,53 +130,6 @@ __device__ __forceinline__ void mma1688(float (&d)[4], const float (&a)[4], floa
         : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
           "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
-// Nibbles 0 and 4 of x as the fp16 numbers n - 8, or nibbles 1 and 5 as 16 (n -
-// 8): ORed into 1024 they are 1024 + n, or 1024 + 16 n, and one subtraction is
-// exact.  (As fp16 subnormals n 2^-24, without it, the tensor core aligned its
-// sum to their exponent field, 2^-14, and scores lost 4 bits.)
-__device__ __forceinline__ uint32_t nib_lo(uint32_t x) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(x));
-    const __half2 h = __hadd2(reinterpret_cast<const __half2&>(r), __float2half2_rn(-1032.0f));
-    return reinterpret_cast<const uint32_t&>(h);
-}
-__device__ __forceinline__ uint32_t nib_hi(uint32_t x) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(x));
-    const __half2 h = __hadd2(reinterpret_cast<const __half2&>(r), __float2half2_rn(-1152.0f));
-    return reinterpret_cast<const uint32_t&>(h);
-}
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-// Nibbles I, I + 1 of x as (n - 8) 16^I, (n - 8) 16^(I + 1) in fp32: each is
-// masked in place and ORed into the mantissa of 2^23, and one packed addition
-// takes `bias`, the pair 2^23 + 8 16^I, .., off.  The pair are neighbours in
-// the MMA's A registers (rows g, g + 8).
-template <int I>
-__device__ __forceinline__ void values2(uint32_t x, uint64_t bias, float& v0, float& v1) {
-    uint32_t u0, u1;
-    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u0) : "r"(x), "n"(0xf << (4 * I)));
-    asm("lop3.b32 %0, %1, %2, 0x4b000000, 0xea;" : "=r"(u1) : "r"(x), "n"(0xf0 << (4 * I)));
-    unpair(f2_add(pair(__uint_as_float(u0), __uint_as_float(u1)), bias), v0, v1);
-}
-// A pair of constants that stays in registers (the compiler would build it anew at every use).
-__device__ __forceinline__ uint64_t held_pair(float lo, float hi) {
-    uint64_t r;
-    asm volatile("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
 // ---------------------------------------------------------- one query row
 // The work is a row of stages -- 4096 / HD tokens of one unit (a query row, a
 // kv head, up to 8 of its query heads) -- cut into equal runs, one for each
@@ -820,10 +762,10 @@ cudaError_t attn_decode(const AttnQ4Args& a, cudaStream_t s) {
 
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s) {
     if (!a.n_q || !a.n_head) return cudaSuccess;
-    const bool one = !a.q_start;
-    if (type == kTypeF32) return one ? attn_decode<float>(a, s) : attn_rows<float>(a, s);
-    if (type == kTypeF16) return one ? attn_decode<__half>(a, s) : attn_rows<__half>(a, s);
-    return one ? attn_decode<__nv_bfloat16>(a, s) : attn_rows<__nv_bfloat16>(a, s);
+    if (a.q_start) return attn_q4_prefill(type, a, s);
+    if (type == kTypeF32) return attn_decode<float>(a, s);
+    if (type == kTypeF16) return attn_decode<__half>(a, s);
+    return attn_decode<__nv_bfloat16>(a, s);
 }
 
 }  // namespace mvb

@@ -240,6 +240,9 @@ struct AttnQ4Args {
     uint64_t out_stride;
 };
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s);
+// attn_q4_prefill.cu : the same for a.q_start's chunks, on tcgen05
+cudaError_t attn_q4_prefill(int type, const AttnQ4Args& a, cudaStream_t s);
+cudaError_t q4_status_take(int* status);
 
 uint64_t attn_smem_bytes(uint64_t hd, uint64_t max_ctx, uint64_t max_pages, int kv_type);
 cudaError_t paged_attn_decode(const AttnArgs& a, cudaStream_t s);
