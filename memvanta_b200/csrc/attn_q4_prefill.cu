@@ -4,21 +4,28 @@
 // A CTA takes NQ tiles of 128 (query row, head) pairs of one sequence and kv
 // head -- 128 / G rows of its G heads -- and walks the sequence's tokens in tiles
 // of NT.  Roles:
-//   NQ x 4 softmax warps (thread = row of its tile = TMEM lane): queries into
-//     shared memory once; then per token tile scores from TMEM, running maximum and
-//     sum, weights back into TMEM;
-//   4 warps that expand the cache: keys to fp16, values to tf32, both exact;
-//   1 warp whose first lane issues the MMAs:
+//   NQ x 4 softmax warps (thread = row of its tile = TMEM lane): per token tile
+//     scores from TMEM, running maximum and sum, weights back into TMEM;
+//   4 or 8 warps that expand the cache: keys to fp16, values to tf32, both exact;
+//   per query tile two warps whose first lanes issue the MMAs:
 //     S (128 x NT) = Q K^T, kind::f16, Q and K from shared memory;
 //     O (128 x HD) += P V, kind::tf32, P from TMEM, V from shared memory.
+//     (An MMA takes its issuing thread some 80 cycles, whatever its size: one
+//     thread for all of them was what bounded a tile, 2,500 cycles.)
+// The scores of tile i + 1 are formed while tile i's weights are: two buffers.
 // A key is (n - 8) d 2^e in fp16, e per token tile such that its largest scale
 // is near 2^7 (smaller scales stay exact down to 2^-20 of it).  Values and weights
 // are tf32, whose exponent range no weight or scale leaves; the value of nibble
 // i carries a factor 16^(i % 4) (kv_q4.cuh), taken off the columns of O at the
-// end.  fp32 queries and their weights go in as two parts of 11 bits each (two
-// MMAs); a half-precision query is one part, and so are its weights, cut to 11
-// bits by the tensor core, with 1 + 2^-12 on them for what the cut takes off
-// on average.
+// end.
+// fp32 queries and their weights go in as two parts of 11 bits each (two
+// MMAs).  The tensor core cuts its running sums to 24 bits at every MMA instead
+// of rounding: summed over a whole context that takes 1.6e-8 an MMA off the
+// outputs (1.5e-4 after 32,768 tokens), so for fp32 queries a tile's outputs start
+// from zero and are added to the total, rounded, by the softmax warps.
+// A half-precision query is one part, and so are its weights, cut to 11 bits
+// by the tensor core, with 1 + 2^-11 0.72 on them for what that takes off on
+// average (mantissas being log-uniform).
 // A masked weight is 0, and 0 times a value that is not finite would not be: such
 // value blocks enter as zeros, and the rows that see one get NaN in its
 // dimensions at the end.
@@ -51,6 +58,12 @@ cudaError_t q4_status_take(int* status) {
 namespace {
 
 constexpr int kRows = 128;  // of a query tile: TMEM lanes
+// Half-precision queries: factor on the weights for what their cut to 11 bits
+// takes off on average, 1 + 2^-11 / (2 ln 2), and its logarithm.
+// fp32: factor on the outputs for the 16 cut sums of a token tile's MMAs
+// (measured: they come out 1.0e-6 short, of 1.2e-6 in all).
+constexpr float kSumCut = 1.0f + 1.0f / 1048576;
+constexpr float kCut = 1.00035225f, kCutLog2 = 5.0811e-4f;
 constexpr int kRing = 4;    // tiles whose exponent and token masks are kept
 
 template <int HD, int NQ, bool TWO>
@@ -64,16 +77,23 @@ struct Pf {
     static constexpr int kOffK = NQ * kParts * kQ;
     static constexpr int kOffV = kOffK + 2 * kK;
     static constexpr int kOffBar = kOffV + 2 * kV;
-    // barriers: k_full, k_empty, v_full, v_empty [2]; s_full, p_full, o_done [NQ]; last
-    static constexpr int kBars = 8 + 3 * NQ + 1;
+    // barriers: k_full, k_empty, v_full, v_empty [2]; s_full, p_full, o_done [NQ][2];
+    // last, t_part, t_free
+    static constexpr int kBars = 8 + 6 * NQ + 3;
     static constexpr int kOffMisc = kOffBar + kBars * 8;
-    // factor 2^-e [kRing], token masks [kRing][2], blocks that are not finite: any
-    // [kRing][2], which tokens [kRing][2][NB]; TMEM base, abort flag, tokens
-    static constexpr int kSmem = kOffMisc + kRing * (4 + 8 + 8 + 8 * NB) + 12 + 1024;
-    static constexpr int kThreads = NQ * 128 + 128 + 32;
-    // TMEM columns of a query tile: scores, then weights (fp32 queries: the first
-    // part in the scores' place, the second beside it), then outputs
-    static constexpr int kCols = 2 * NT + HD;
+    // exponents of the query rows [NQ][128]; factor 2^-e [kRing], token masks
+    // [kRing][2], blocks that are not finite: any [kRing][2], which tokens
+    // [kRing][2][NB]; TMEM base, abort flag, tokens
+    static constexpr int kSmem = kOffMisc + NQ * kRows * 4 + kRing * (4 + 8 + 8 + 8 * NB) + 12 + 1024;
+    static constexpr int kExpand = NQ == 2 ? 4 : 8;  // warps
+    static constexpr int kThreads = NQ * 128 + kExpand * 32 + 2 * NQ * 32;
+    // TMEM columns of a query tile: two buffers of NT scores, taken by the
+    // weights (their first part) of the same token tile; fp32: two of the weights'
+    // second part, and a tile's outputs, OT columns at a time; outputs HD.
+    static constexpr int OT = HD == 256 ? 128 : HD;
+    static constexpr int kOffL = 2 * NT, kOffT = 4 * NT;
+    static constexpr int kOffO = TWO ? kOffT + OT : 2 * NT;
+    static constexpr int kCols = kOffO + HD;
     static constexpr uint32_t kTmem = NQ * kCols <= 256 ? 256 : 512;
     static_assert(NQ * kCols <= 512, "tensor memory");
     static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -139,12 +159,13 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
     auto k_empty = [&](int s) { return bars + 16 + 8 * s; };
     auto v_full = [&](int s) { return bars + 32 + 8 * s; };
     auto v_empty = [&](int s) { return bars + 48 + 8 * s; };
-    auto s_full = [&](int q) { return bars + 64 + 8 * q; };
-    auto p_full = [&](int q) { return bars + 64 + 8 * (NQ + q); };
-    auto o_done = [&](int q) { return bars + 64 + 8 * (2 * NQ + q); };
-    const uint32_t last_bar = bars + 64 + 8 * 3 * NQ;
-    float* k_back = reinterpret_cast<float*>(sm + C::kOffMisc);                    // [kRing] 2^-e
-    uint32_t* there = reinterpret_cast<uint32_t*>(sm + C::kOffMisc + 4 * kRing);   // [kRing][2]
+    auto s_full = [&](int q, int i) { return bars + 64 + 8 * (2 * q + (i & 1)); };
+    auto p_full = [&](int q, int i) { return bars + 64 + 8 * (2 * NQ + 2 * q + (i & 1)); };
+    auto o_done = [&](int q, int i) { return bars + 64 + 8 * (4 * NQ + 2 * q + (i & 1)); };
+    const uint32_t last_bar = bars + 64 + 8 * 6 * NQ, t_part = last_bar + 8, t_free = last_bar + 16;
+    int* q_exp = reinterpret_cast<int*>(sm + C::kOffMisc);                         // [NQ][128]
+    float* k_back = reinterpret_cast<float*>(q_exp + NQ * kRows);                  // [kRing] 2^-e
+    uint32_t* there = reinterpret_cast<uint32_t*>(k_back + kRing);                 // [kRing][2]
     uint32_t* any_bad = there + 2 * kRing;                                         // [kRing][2]
     uint32_t* bad_tokens = any_bad + 2 * kRing;                                    // [kRing][2][NB]
     uint32_t* tmem_at = bad_tokens + 2 * kRing * NB;
@@ -153,73 +174,87 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(k_full(i), 128);
-            tc::mbar_init(v_full(i), 128);
-            tc::mbar_init(k_empty(i), 1);
-            tc::mbar_init(v_empty(i), 1);
+            tc::mbar_init(k_full(i), C::kExpand * 32);
+            tc::mbar_init(v_full(i), C::kExpand * 32);
+            tc::mbar_init(k_empty(i), NQ);
+            tc::mbar_init(v_empty(i), NQ);
         }
-        for (int q = 0; q < NQ; ++q) {
-            tc::mbar_init(s_full(q), 2);  // the MMAs' commit, and their issuer
-            tc::mbar_init(p_full(q), 128);
-            tc::mbar_init(o_done(q), 1);
-        }
-        tc::mbar_init(last_bar, 1);
+        for (int q = 0; q < NQ; ++q)
+            for (int i = 0; i < 2; ++i) {
+                tc::mbar_init(s_full(q, i), 2);  // the MMAs' commit, and their issuer
+                tc::mbar_init(p_full(q, i), 128);
+                tc::mbar_init(o_done(q, i), 1);
+            }
+        tc::mbar_init(last_bar, 2 * NQ);
+        tc::mbar_init(t_part, 1);
+        tc::mbar_init(t_free, 128);  // a tile's first OT columns are taken out
         tc::mbar_fence_init();
         *abort_flag = 0;
         *most = 0;
     }
-    constexpr int kMmaWarp = NQ * 4 + 4;
+    constexpr int kMmaWarp = NQ * 4 + C::kExpand;
     if (warp == kMmaWarp) {
         tc::tmem_alloc(tc::smem_u32(tmem_at), C::kTmem);
         tc::tmem_relinquish();
     }
     __syncthreads();
 
-    // ---- queries: thread m of tile q holds row m / nh, head m % nh
-    const int q_of = warp / 4, m = (warp % 4) * 32 + lane;
-    int ctx = 0;
-    int64_t my_row = -1;
-    int my_head = 0;
-    float c_row = 0.0f;
-    if (warp < NQ * 4) {
-        const int64_t r = row0 + q_of * p.rpt + m / nh;
-        if (m / nh < p.rpt && r < seq1) {
-            my_row = r;
-            my_head = h0 + m % nh;
-            ctx = max(0, min(a.ctx_len[r], (int)a.max_ctx));
-        }
-        const T* src = static_cast<const T*>(a.q) + max(my_row, (int64_t)0) * (int64_t)a.q_stride + (int64_t)my_head * HD;
-        float mx = 0.0f;
-#pragma unroll 4
-        for (int u = 0; u < HD / 8; ++u) {
-            float x[8];
-            load_n<8, true>(src + 8 * u, x);
+    // ---- queries into shared memory, 8 lanes to a row: row m of tile q is query
+    // row m / nh, head m % nh
+    if (warp < kMmaWarp) {
+        constexpr int kPer = HD / 64;  // 8-dimension units of a lane
+#pragma unroll 1
+        for (int r = warp * 4 + lane / 8; r < NQ * kRows; r += kMmaWarp * 4) {
+            const int tile = r / kRows, m = r % kRows, u0 = lane % 8;
+            const int64_t row = row0 + tile * p.rpt + m / nh;
+            const bool there_is = m / nh < p.rpt && row < seq1;
+            const T* src = static_cast<const T*>(a.q) + (there_is ? row * (int64_t)a.q_stride + (int64_t)(h0 + m % nh) * HD : 0);
+            float x[kPer][8], mx = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[i]));
-        }
-        // times 2^e: the largest below 2^15
-        const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
-        const float up = my_row >= 0 ? pow2i(e) : 0.0f;
-        c_row = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
-        uint8_t* dst = sm + q_of * C::kParts * C::kQ;
-#pragma unroll 2
-        for (int u = 0; u < HD / 8; ++u) {
-            float x[8], lo[8];
-            load_n<8, true>(src + 8 * u, x);
+            for (int k = 0; k < kPer; ++k) {
+                load_n<8, true>(src + 8 * (u0 + 8 * k), x[k]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = my_row >= 0 ? x[i] * up : 0.0f;
-                lo[i] = x[i] - __half2float(__float2half_rn(x[i]));
+                for (int i = 0; i < 8; ++i) {
+                    if (!there_is) x[k][i] = 0.0f;
+                    mx = fmaxf(mx, fabsf(x[k][i]));
+                }
             }
-            // dims of a unit in the order of the expanded keys: 0 4 1 5 2 6 3 7
-            uint8_t* at = dst + (u / 8) * kRows * 128 + sw128(m, u % 8);
-            *reinterpret_cast<uint4*>(at) = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]),
-                                                       pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
-            if constexpr (kTwo)
-                *reinterpret_cast<uint4*>(at + C::kQ) = make_uint4(pack_half2(lo[0], lo[4]), pack_half2(lo[1], lo[5]),
-                                                                   pack_half2(lo[2], lo[6]), pack_half2(lo[3], lo[7]));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            // times 2^e: the largest below 2^15
+            const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+            const float up = pow2i(e);
+            if (u0 == 0) q_exp[r] = e;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                float lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[k][i] *= up;
+                    lo[i] = x[k][i] - __half2float(__float2half_rn(x[k][i]));
+                }
+                // dims of a unit in the order of the expanded keys: 0 4 1 5 2 6 3 7
+                uint8_t* at = sm + tile * C::kParts * C::kQ + k * kRows * 128 + sw128(m, u0);
+                *reinterpret_cast<uint4*>(at) = make_uint4(pack_half2(x[k][0], x[k][4]), pack_half2(x[k][1], x[k][5]),
+                                                           pack_half2(x[k][2], x[k][6]), pack_half2(x[k][3], x[k][7]));
+                if constexpr (kTwo)
+                    *reinterpret_cast<uint4*>(at + C::kQ) = make_uint4(pack_half2(lo[0], lo[4]), pack_half2(lo[1], lo[5]),
+                                                                       pack_half2(lo[2], lo[6]), pack_half2(lo[3], lo[7]));
+            }
         }
         tc::fence_proxy_async_smem();
+    }
+    // softmax thread m of tile q holds that row
+    const int q_of = warp / 4, m_of = (warp % 4) * 32 + lane;
+    int ctx = 0, my_head = 0;
+    int64_t my_row = -1;
+    if (warp < NQ * 4) {
+        const int64_t r = row0 + q_of * p.rpt + m_of / nh;
+        if (m_of / nh < p.rpt && r < seq1) {
+            my_row = r;
+            my_head = h0 + m_of % nh;
+            ctx = max(0, min(a.ctx_len[r], (int)a.max_ctx));
+        }
         const int top = __reduce_max_sync(0xffffffffu, ctx);
         if (lane == 0 && top) atomicMax(most, top);
     }
@@ -229,72 +264,57 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
     const uint32_t tmem = *tmem_at;
     const int tokens = *most, tiles = (tokens + NT - 1) / NT;
 
-    if (warp == kMmaWarp) {
-        // ------------------------------------------------------ MMA issuer
+    if (warp >= kMmaWarp) {
+        // ----------------------------------------------------- MMA issuers
+        const int q = (warp - kMmaWarp) % NQ;
+        const uint32_t t = tmem + q * C::kCols;
+        auto wait = [&](uint32_t bar, int parity, int site) {
+            if (!tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site)) return false;
+            tc::tc_fence_after();
+            return true;
+        };
         if (lane == 0 && tiles) {
-            constexpr uint32_t id_qk = idesc(0, kRows, NT), id_pv = idesc(2, kRows, HD);
-            auto wait = [&](uint32_t bar, int parity, int site) {
-                return tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site);
-            };
-            auto scores = [&](int q, int i) {
-                const uint32_t kb = sb + C::kOffK + (i & 1) * C::kK, qb = sb + q * C::kParts * C::kQ;
-                const uint32_t d = tmem + q * C::kCols;
+            if (warp - kMmaWarp < NQ) {
+                // scores, into the buffer whose weights, of two tiles before, have been multiplied
+                constexpr uint32_t id = idesc(0, kRows, NT);
+                const uint32_t qb = sb + q * C::kParts * C::kQ;
+                for (int i = 0; i < tiles; ++i) {
+                    if (!wait(k_full(i & 1), i >> 1, 40)) break;
+                    if (i >= 2 && !wait(o_done(q, i), (i - 2) >> 1, 41)) break;
+                    const uint32_t kb = sb + C::kOffK + (i & 1) * C::kK, d = t + (i & 1) * NT;
 #pragma unroll
-                for (int part = 0; part < C::kParts; ++part)
+                    for (int part = 0; part < C::kParts; ++part)
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        mma_f16_ss(d, tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
-                                   tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id_qk, part || k);
-                tc::mma_commit(s_full(q));
-                tc::mbar_arrive(s_full(q));
-            };
-            auto outputs = [&](int q, int i) {
-                const uint32_t vb = sb + C::kOffV + (i & 1) * C::kV;
-                const uint32_t s = tmem + q * C::kCols, d = s + 2 * NT;
-#pragma unroll
-                for (int part = 0; part < C::kParts; ++part)
-#pragma unroll
-                    for (int k = 0; k < NT / 8; ++k)
-                        mma_tf32_ts(d, s + (kTwo ? part * NT : NT) + 8 * k,
-                                    tc::sdesc_kmajor_sw128(vb + (k / 4) * HD * 128) + 2 * (k % 4), id_pv,
-                                    i || part || k);
-                tc::mma_commit(o_done(q));
-            };
-            bool ok = wait(k_full(0), 0, 40);
-            if (ok) {
-                tc::tc_fence_after();
-                for (int q = 0; q < NQ; ++q) scores(q, 0);
-                tc::mma_commit(k_empty(0));
-            }
-            for (int i = 0; ok && i < tiles; ++i) {
-                const bool more = i + 1 < tiles;
-                for (int q = 0; ok && q < NQ; ++q) {
-                    // the weights are in TMEM, and so the scores have been read
-                    ok = wait(p_full(q), i, 41);
-                    if constexpr (!kTwo) {
-                        if (ok && more && q == 0) ok = wait(k_full((i + 1) & 1), (i + 1) >> 1, 42);
-                        if (ok && more) {
-                            tc::tc_fence_after();
-                            scores(q, i + 1);
-                            if (q == NQ - 1) tc::mma_commit(k_empty((i + 1) & 1));
-                        }
-                    }
-                    if (ok && q == 0) ok = wait(v_full(i & 1), i >> 1, 43);
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    outputs(q, i);
-                    if (q == NQ - 1) tc::mma_commit(v_empty(i & 1));
+                        for (int k = 0; k < HD / 16; ++k)
+                            mma_f16_ss(d, tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
+                                       tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id, part || k);
+                    tc::mma_commit(s_full(q, i));
+                    tc::mbar_arrive(s_full(q, i));
+                    tc::mma_commit(k_empty(i & 1));
                 }
-                if constexpr (kTwo) {
-                    // the first weights' part lies where the next scores go
-                    if (ok && more) ok = wait(k_full((i + 1) & 1), (i + 1) >> 1, 44);
-                    for (int q = 0; ok && more && q < NQ; ++q) {
-                        ok = wait(o_done(q), i, 45);
+            } else {
+                // outputs, OT columns at a time for fp32
+                constexpr uint32_t id = idesc(2, kRows, kTwo ? C::OT : HD);
+                constexpr int kTurns = kTwo ? HD / C::OT : 1;
+                bool ok = true;
+                for (int i = 0; ok && i < tiles; ++i) {
+                    ok = wait(v_full(i & 1), i >> 1, 42) && wait(p_full(q, i), i >> 1, 43);
+#pragma unroll
+                    for (int turn = 0; turn < kTurns; ++turn) {
+                        if (turn && ok) ok = wait(t_free, i, 44);  // the columns before are taken out
                         if (!ok) break;
-                        tc::tc_fence_after();
-                        scores(q, i + 1);
-                        if (q == NQ - 1) tc::mma_commit(k_empty((i + 1) & 1));
+                        const uint32_t vb = sb + C::kOffV + (i & 1) * C::kV + turn * C::OT * 128;
+                        const uint32_t d = t + (kTwo ? C::kOffT : C::kOffO);
+#pragma unroll
+                        for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+                            for (int k = 0; k < NT / 8; ++k)
+                                mma_tf32_ts(d, t + part * C::kOffL + (i & 1) * NT + 8 * k,
+                                            tc::sdesc_kmajor_sw128(vb + (k / 4) * HD * 128) + 2 * (k % 4), id,
+                                            (!kTwo && i) || part || k);
+                        tc::mma_commit(turn + 1 < kTurns ? t_part : o_done(q, i));
                     }
+                    if (ok) tc::mma_commit(v_empty(i & 1));
                 }
             }
             // every MMA issued has completed before TMEM is released
@@ -303,97 +323,113 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         }
     } else if (warp >= NQ * 4) {
         // ------------------------------------------------ cache expansion
-        constexpr int kGroups = NT / 32, kSplit = 4 / kGroups;  // warps per 32 tokens
-        constexpr int W = HD / 8 / kSplit;                      // words of a token that a lane takes
-        const int w4 = warp - NQ * 4, grp = w4 % kGroups, first = w4 / kGroups * W;
+        constexpr int kGroups = NT / 32, kSplit = C::kExpand / kGroups;  // warps per 32 tokens
+        constexpr int W = HD / 8 / kSplit;                               // words of a token that a lane takes
+        static_assert(W % NB == 0 || NB % W == 0, "a warp's words start at a block that its lanes share");
+        const int w8 = warp - NQ * 4, grp = w8 % kGroups, first = w8 / kGroups * W;
+        const int b0 = first % NB, t0 = first / NB;  // block and quarter of the first word
         const int32_t* table = a.block_table + (int64_t)seq * (int64_t)a.max_pages;
         const uint32_t page = (uint32_t)a.page;
-        static_assert(W % NB == 0, "a lane's word k is of block k % NB");
         // this lane's words, its token's scales, the other group's key scales
-        uint32_t kw[W], vw[W], ks[NB / 2], vs[NB / 2], ks_other[NB / 2], mask;
-        auto slot_of = [&](uint32_t tok, bool& ok) -> uint64_t {
+        struct Raw {
+            uint32_t kw[W], vw[W], ks[NB / 2], vs[NB / 2], ks_other[NB / 2], mask;
+        };
+        // slots of this lane's token of the tile after the fetched one, looked up a tile ahead
+        uint32_t slot_own = 0, slot_other = 0;
+        bool ok_own = false, ok_other = false;
+        auto slot_of = [&](uint32_t tok, bool& ok) -> uint32_t {
             ok = false;
             if (tok >= (uint32_t)tokens) return 0;
             const uint32_t pi = __umulhi(tok << 1, p.page_mul) >> p.page_shift, pg = (uint32_t)table[pi];
             ok = pg < (uint32_t)a.n_pages;
             return ok ? (pg * (uint32_t)H + (uint32_t)kvh) * page + (tok - pi * page) : 0;
         };
-        auto scales = [&](const uint16_t* pool, uint64_t slot, bool ok, uint32_t (&out)[NB / 2]) {
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(pool) + slot * (NB / 2);
+        auto look_up = [&](int i) {
+            slot_own = slot_of((uint32_t)i * NT + 32 * grp + lane, ok_own);
+            if constexpr (kGroups == 2) slot_other = slot_of((uint32_t)i * NT + 32 * (grp ^ 1) + lane, ok_other);
+        };
+        auto scales = [&](const uint16_t* pool, uint32_t slot, bool ok, uint32_t (&out)[NB / 2]) {
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(pool) + (uint64_t)slot * (NB / 2);
 #pragma unroll
             for (int k = 0; k < NB / 2; ++k) out[k] = ok ? src[k] : 0u;
         };
-        auto fetch = [&](int i) {
-            bool ok;
-            uint64_t slot = slot_of((uint32_t)i * NT + 32 * grp + lane, ok);
-            mask = __ballot_sync(0xffffffffu, ok);
-            scales(a.k_scales, slot, ok, ks);
-            scales(a.v_scales, slot, ok, vs);
-            const uint8_t* kp = a.k_pages + slot * (HD / 2) + first * 4;
-            const uint8_t* vp = a.v_pages + slot * (HD / 2) + first * 4;
+        auto words = [&](const uint8_t* pool, uint32_t (&out)[W]) {
+            const uint8_t* src = pool + (uint64_t)slot_own * (HD / 2) + first * 4;
+            if constexpr (W == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(src);
+                out[0] = x.x, out[1] = x.y;
+            } else {
 #pragma unroll
-            for (int k = 0; k < W; k += 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(kp + 4 * k);
-                const uint4 y = *reinterpret_cast<const uint4*>(vp + 4 * k);
-                kw[k] = x.x, kw[k + 1] = x.y, kw[k + 2] = x.z, kw[k + 3] = x.w;
-                vw[k] = y.x, vw[k + 1] = y.y, vw[k + 2] = y.z, vw[k + 3] = y.w;
-            }
-            if constexpr (kGroups == 2) {
-                slot = slot_of((uint32_t)i * NT + 32 * (grp ^ 1) + lane, ok);
-                scales(a.k_scales, slot, ok, ks_other);
+                for (int k = 0; k < W; k += 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(src + 4 * k);
+                    out[k] = x.x, out[k + 1] = x.y, out[k + 2] = x.z, out[k + 3] = x.w;
+                }
             }
         };
-        auto scale = [](const uint32_t (&sc)[NB / 2], int b) {
-            return __uint_as_float(b % 2 ? sc[b / 2] & 0xffff0000u : sc[b / 2] << 16);
+        auto fetch = [&](Raw& r) {
+            r.mask = __ballot_sync(0xffffffffu, ok_own);
+            scales(a.k_scales, slot_own, ok_own, r.ks);
+            scales(a.v_scales, slot_own, ok_own, r.vs);
+            words(a.k_pages, r.kw);
+            words(a.v_pages, r.vw);
+            if constexpr (kGroups == 2) scales(a.k_scales, slot_other, ok_other, r.ks_other);
+        };
+        // scale of the block of word k
+        auto scale = [&](const uint32_t (&sc)[NB / 2], int k) {
+            const int b = k % NB;
+            uint32_t w = sc[b / 2];
+            if constexpr (W < NB) w = b0 ? sc[b / 2 + W / 2] : w;
+            return __uint_as_float(b % 2 ? w & 0xffff0000u : w << 16);
         };
         auto finite = [](uint32_t bits) { return (bits & 0x7f80u) != 0x7f80u; };
         const uint64_t bias0 = held_pair(-8388616.0f, -8388736.0f), bias1 = held_pair(-8390656.0f, -8421376.0f);
         uint32_t lane_at[8];  // of this lane's token in row d of the values, d % 8 = i
 #pragma unroll
         for (int i = 0; i < 8; ++i) lane_at[i] = (uint32_t)((((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
-        bool ok = true;
-        if (tiles) fetch(0);
-        for (int i = 0; i < tiles; ++i) {
+        // expands tile i from r, fetching tile i + 1 into `ahead` meanwhile
+        auto expand = [&](const Raw& r, Raw& ahead, int i) -> bool {
             const int s = i & 1;
+            if (i + 1 < tiles) {
+                fetch(ahead);
+                look_up(i + 2);
+            }
             // ---- keys
-            uint32_t dm = 0;
+            uint32_t dm = 0, bad = 0;
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                const uint32_t x = (ks[k / 2] >> (k % 2 * 16)) & 0x7fffu;
+                const uint32_t x = (r.ks[k / 2] >> (k % 2 * 16)) & 0x7fffu;
                 dm = max(dm, finite(x) ? x : 0u);
                 if constexpr (kGroups == 2) {
-                    const uint32_t y = (ks_other[k / 2] >> (k % 2 * 16)) & 0x7fffu;
+                    const uint32_t y = (r.ks_other[k / 2] >> (k % 2 * 16)) & 0x7fffu;
                     dm = max(dm, finite(y) ? y : 0u);
                 }
+                bad |= finite(r.vs[k / 2] >> (k % 2 * 16)) ? 0u : 1u << k;  // value blocks that are not finite
             }
             dm = __reduce_max_sync(0xffffffffu, dm);
+            const bool some = __any_sync(0xffffffffu, bad);
             const int e = max(-126, min(126, 6 - ((int)(dm >> 7) - 127)));
             const float up = pow2i(e);
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, &g_q4_status, 47));
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu,
+                            tc::mbar_wait(k_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, &g_q4_status, 47)))
+                return false;
             uint8_t* kd = sm + C::kOffK + s * C::kK;
             const int row = grp * 32 + lane;
 #pragma unroll
             for (int k = 0; k < W; ++k) {
-                const int t = first / NB + k / NB, b = k % NB;
-                const float d = scale(ks, b) * up;
+                const int b = b0 + k % NB, t = t0 + k / NB;
+                const float d = scale(r.ks, k) * up;
                 const __half2 d2 = __float2half2_rn(d), d16 = __float2half2_rn(d * 0.0625f);
                 auto mul = [](uint32_t x, __half2 y) {
-                    const __half2 r = __hmul2(reinterpret_cast<const __half2&>(x), y);
-                    return reinterpret_cast<const uint32_t&>(r);
+                    const __half2 v = __hmul2(reinterpret_cast<const __half2&>(x), y);
+                    return reinterpret_cast<const uint32_t&>(v);
                 };
-                const uint32_t x = kw[k], x8 = x >> 8;
+                const uint32_t x = r.kw[k], x8 = x >> 8;
                 *reinterpret_cast<uint4*>(kd + (b / 2) * NT * 128 + sw128(row, (b % 2) * 4 + t)) =
                     make_uint4(mul(nib_lo(x), d2), mul(nib_hi(x), d16), mul(nib_lo(x8), d2), mul(nib_hi(x8), d16));
             }
-            // value blocks that are not finite
-            uint32_t bad = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) bad |= finite(vs[b / 2] >> (b % 2 * 16)) ? 0u : 1u << b;
-            const bool some = __any_sync(0xffffffffu, bad);
-            if (w4 < kGroups) {
+            if (w8 < kGroups) {
                 const int at = (i % kRing) * 2 + grp;
-                if (lane == 0) k_back[i % kRing] = pow2i(-e), there[at] = mask, any_bad[at] = some;
+                if (lane == 0) k_back[i % kRing] = pow2i(-e), there[at] = r.mask, any_bad[at] = some;
                 if (some)
                     for (int b = 0; b < NB; ++b) {
                         const uint32_t which = __ballot_sync(0xffffffffu, bad >> b & 1u);
@@ -403,17 +439,19 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             tc::fence_proxy_async_smem();
             tc::mbar_arrive(k_full(s));
             // ---- values
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(v_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, &g_q4_status, 48));
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu,
+                            tc::mbar_wait(v_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, &g_q4_status, 48)))
+                return false;
             uint8_t* vd = sm + C::kOffV + s * C::kV + grp * HD * 128;
 #pragma unroll
             for (int k = 0; k < W; ++k) {
-                const int t = first / NB + k / NB, b = k % NB;
-                const float d = bad >> b & 1u ? 0.0f : scale(vs, b);
+                const int b = b0 + k % NB, t = t0 + k / NB;
+                float d = scale(r.vs, k);
+                if (some && (bad >> b & 1u)) d = 0.0f;
                 uint8_t* dst = vd + (32 * b + 8 * t) * 128;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint32_t x = half ? vw[k] >> 16 : vw[k];
+                    const uint32_t x = half ? r.vw[k] >> 16 : r.vw[k];
                     float v[4];
                     values2<0>(x, bias0, v[0], v[1]);
                     values2<2>(x, bias1, v[2], v[3]);
@@ -424,21 +462,63 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             }
             tc::fence_proxy_async_smem();
             tc::mbar_arrive(v_full(s));
-            if (i + 1 < tiles) fetch(i + 1);
+            return true;
+        };
+        Raw ra, rb;
+        if (tiles) {
+            look_up(0);
+            fetch(ra);
+            look_up(1);
+        }
+        for (int i = 0; i < tiles; i += 2) {
+            if (!expand(ra, rb, i)) break;
+            if (i + 1 < tiles && !expand(rb, ra, i + 1)) break;
         }
     } else {
         // ------------------------------------------------------- softmax
         const uint32_t tm = tmem + q_of * C::kCols + ((uint32_t)(warp % 4) << 21);  // this warp's 32 lanes
+        const float c_row = fmaxf(a.scale * 1.44269504088896341f * pow2i(-q_exp[q_of * kRows + m_of]), 1e-37f);
         float m_run = -INFINITY, l = 0.0f;
         uint32_t bad = 0;  // blocks of dimensions in which this row sees values that are not finite
         bool ok = true;
+        auto wait = [&](uint32_t bar, int parity, int site) {
+            const bool got = __all_sync(0xffffffffu, tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site));
+            if (got) tc::tc_fence_after();
+            return got;
+        };
+        // fp32: adds tile i's outputs to the total, OT columns at a time
+        auto add_tile = [&](int i) {
+#pragma unroll 1
+            for (int turn = 0; turn < HD / C::OT; ++turn) {
+                if (turn + 1 < HD / C::OT ? !wait(t_part, i, 52) : !wait(o_done(q_of, i), i >> 1, 50)) return false;
+#pragma unroll 1
+                for (int j = 0; j < C::OT / 32; ++j) {
+                    const uint32_t at = tm + C::kOffO + turn * C::OT + 32 * j;
+                    uint32_t x[32], o[32];
+                    tc::tmem_ld32(tm + C::kOffT + 32 * j, x);
+                    if (i) tc::tmem_ld32(at, o);
+                    tc::tmem_wait_ld();
+                    if (i)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            x[k] = __float_as_uint(__uint_as_float(x[k]) + __uint_as_float(o[k]));
+                    tc::tmem_st32(at, x);
+                }
+                if (turn + 1 < HD / C::OT) {  // the next columns may come
+                    tc::tc_fence_before();
+                    tc::mbar_arrive(t_free);
+                }
+            }
+            tc::tmem_wait_st();
+            return true;
+        };
         for (int i = 0; ok && i < tiles; ++i) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full(q_of), (uint32_t)i & 1u, abort_flag, &g_q4_status, 49));
+            ok = wait(s_full(q_of, i), i >> 1, 49);
             if (!ok) break;
-            tc::tc_fence_after();
+            const uint32_t ts = tm + (i & 1) * NT;  // this tile's scores, and weights
             uint32_t s[NT / 32][32];
 #pragma unroll
-            for (int j = 0; j < NT / 32; ++j) tc::tmem_ld32(tm + 32 * j, s[j]);
+            for (int j = 0; j < NT / 32; ++j) tc::tmem_ld32(ts + 32 * j, s[j]);
             tc::tmem_wait_ld();
             const float c = c_row * k_back[i % kRing];
             const int left = ctx - i * NT;  // of this row's tokens
@@ -462,74 +542,80 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                 if (any_bad[(i % kRing) * 2 + j])
                     for (int b = 0; b < NB; ++b)
                         if (bad_tokens[((i % kRing) * 2 + j) * NB + b] & msk[j]) bad |= 1u << b;
-            float mx = __uint_as_float(s[0][0]);
+            // four chains each for the maximum and the sum: one is 64 dependent steps
+            float mx4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx4[k] = __uint_as_float(s[0][k]);
 #pragma unroll
             for (int j = 0; j < NT / 32; ++j)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(s[j][k]));
-            mx *= c;
-            // the weights of the tile before have been multiplied: their place
-            // is free, and the outputs may be touched
-            if (i) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done(q_of), (uint32_t)(i - 1) & 1u, abort_flag, &g_q4_status, 50));
-                if (!ok) break;
-                tc::tc_fence_after();
-            }
+                for (int k = 0; k < 32; ++k) mx4[k % 4] = fmaxf(mx4[k % 4], __uint_as_float(s[j][k]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c;
             // the reference m follows the maximum once that is 2^8 above it
-            if (__any_sync(0xffffffffu, mx > m_run + 8.0f)) {
-                const bool mine = mx > m_run + 8.0f;
-                const float alpha = mine ? ex2(m_run - mx) : 1.0f;
-                if (mine) m_run = mx;
-                l *= alpha;
-                if (i) {
+            const bool move = mx > m_run + 8.0f;
+            const float alpha = move ? ex2(m_run - mx) : 1.0f;
+            if (move) m_run = mx;
+            l *= alpha;
+            const float m_use = (m_run == -INFINITY ? 0.0f : m_run) - (kTwo ? 0.0f : kCutLog2);
+            const uint64_t cc = pair(c, c), mm = pair(-m_use, -m_use);
+            uint64_t l2[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < NT / 16; ++j) {
+                uint32_t w[16], w2[16];
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    const uint32_t* sp = &s[j / 2][j % 2 * 16 + k];
+                    float x0, x1;
+                    unpair(tc::f2_fma(pair(__uint_as_float(sp[0]), __uint_as_float(sp[1])), cc, mm), x0, x1);
+                    x0 = ex2(x0), x1 = ex2(x1);
+                    l2[k / 2 % 2] = f2_add(l2[k / 2 % 2], pair(x0, x1));
+                    w[k] = __float_as_uint(x0), w[k + 1] = __float_as_uint(x1);
+                    if constexpr (kTwo) {
+                        w[k] &= 0xffffe000u, w[k + 1] &= 0xffffe000u;  // 11 bits
+                        w2[k] = __float_as_uint(x0 - __uint_as_float(w[k]));
+                        w2[k + 1] = __float_as_uint(x1 - __uint_as_float(w[k + 1]));
+                    }
+                }
+                tc::tmem_st16(ts + 16 * j, w);
+                if constexpr (kTwo) tc::tmem_st16(ts + C::kOffL + 16 * j, w2);
+            }
+            float x0, x1;
+            unpair(f2_add(l2[0], l2[1]), x0, x1);
+            l += x0 + x1;
+            // the outputs up to the tile before are summed; on the new reference
+            if (i) {
+                if constexpr (kTwo) ok = add_tile(i - 1);
+                else ok = wait(o_done(q_of, i - 1), (i - 1) >> 1, 50);
+                if (!ok) break;
+                if (__any_sync(0xffffffffu, move)) {
 #pragma unroll 1
                     for (int j = 0; j < HD / 32; ++j) {
                         uint32_t o[32];
-                        tc::tmem_ld32(tm + 2 * NT + 32 * j, o);
+                        tc::tmem_ld32(tm + C::kOffO + 32 * j, o);
                         tc::tmem_wait_ld();
 #pragma unroll
                         for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                        tc::tmem_st32(tm + 2 * NT + 32 * j, o);
+                        tc::tmem_st32(tm + C::kOffO + 32 * j, o);
                     }
                 }
-            }
-            // half-precision queries: weights 1 + 2^-12 larger, taken off the sum below
-            const float m_use = (m_run == -INFINITY ? 0.0f : m_run) - (kTwo ? 0.0f : 3.52176e-4f);
-#pragma unroll
-            for (int j = 0; j < NT / 32; ++j) {
-                uint32_t w[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    const float pr = ex2(fmaf(__uint_as_float(s[j][k]), c, -m_use));
-                    l += pr;
-                    if constexpr (kTwo) {
-                        const uint32_t hi = __float_as_uint(pr) & 0xffffe000u;  // 11 bits
-                        w[k] = __float_as_uint(pr - __uint_as_float(hi));
-                        s[j][k] = hi;
-                    } else {
-                        s[j][k] = __float_as_uint(pr);
-                    }
-                }
-                tc::tmem_st32(tm + (kTwo ? 0 : NT) + 32 * j, s[j]);
-                if constexpr (kTwo) tc::tmem_st32(tm + NT + 32 * j, w);
             }
             tc::tmem_wait_st();
             tc::tc_fence_before();
-            tc::mbar_arrive(p_full(q_of));
+            tc::mbar_arrive(p_full(q_of, i));
         }
         // ---- outputs
         if (ok && tiles) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done(q_of), (uint32_t)(tiles - 1) & 1u, abort_flag, &g_q4_status, 51));
-            tc::tc_fence_after();
+            if constexpr (kTwo) ok = add_tile(tiles - 1);
+            else ok = wait(o_done(q_of, tiles - 1), (tiles - 1) >> 1, 51);
         }
         if (ok) {
-            const float inv = l == 0.0f ? 0.0f : (kTwo ? 1.0f : 1.000244140625f) / l;
+            const float inv = l == 0.0f ? 0.0f : (kTwo ? kSumCut : kCut) / l;
             T* out = static_cast<T*>(a.out) + max(my_row, (int64_t)0) * (int64_t)a.out_stride + (int64_t)my_head * HD;
 #pragma unroll 1
             for (int j = 0; j < HD / 32; ++j) {
                 uint32_t o[32];
                 if (tiles) {
-                    tc::tmem_ld32(tm + 2 * NT + 32 * j, o);
+                    tc::tmem_ld32(tm + C::kOffO + 32 * j, o);
                     tc::tmem_wait_ld();
                 }
 #pragma unroll
@@ -575,8 +661,12 @@ cudaError_t prefill_of(const PfArgs& p, cudaStream_t s) {
     // still gives every SM a CTA
     const uint64_t units = p.a.n_seq * p.a.n_head_kv * (uint64_t)p.chunks;
     const bool two = ((p.a.max_q + (uint64_t)(2 * p.rpt) - 1) / (uint64_t)(2 * p.rpt)) * units >= 148;
-    if (p.a.hd == 64) return two ? launch_prefill<T, 64, 2>(p, s) : launch_prefill<T, 64, 1>(p, s);
-    if (p.a.hd == 128) return two ? launch_prefill<T, 128, 2>(p, s) : launch_prefill<T, 128, 1>(p, s);
+    if constexpr (sizeof(T) == 2) {  // (fp32: tensor memory holds one)
+        if (two && p.a.hd == 64) return launch_prefill<T, 64, 2>(p, s);
+        if (two && p.a.hd == 128) return launch_prefill<T, 128, 2>(p, s);
+    }
+    if (p.a.hd == 64) return launch_prefill<T, 64, 1>(p, s);
+    if (p.a.hd == 128) return launch_prefill<T, 128, 1>(p, s);
     return launch_prefill<T, 256, 1>(p, s);
 }
 
