@@ -7,11 +7,9 @@
 //   NQ x 4 softmax warps (thread = row of its tile = TMEM lane): per token tile
 //     scores from TMEM, running maximum and sum, weights back into TMEM;
 //   4 or 8 warps that expand the cache: keys to fp16, values to tf32, both exact;
-//   per query tile two warps whose first lanes issue the MMAs:
+//   per query tile two warps that issue the MMAs:
 //     S (128 x NT) = Q K^T, kind::f16, Q and K from shared memory;
 //     O (128 x HD) += P V, kind::tf32, P from TMEM, V from shared memory.
-//     (An MMA takes its issuing thread some 80 cycles, whatever its size: one
-//     thread for all of them was what bounded a tile, 2,500 cycles.)
 // The scores of tile i + 1 are formed while tile i's weights are: two buffers.
 // A key is (n - 8) d 2^e in fp16, e per token tile such that its largest scale
 // is near 2^7 (smaller scales stay exact down to 2^-20 of it).  Values and weights
@@ -114,18 +112,27 @@ __host__ __device__ constexpr uint32_t idesc(int kind_ab, int M, int N) {
     return (1u << 4) | ((uint32_t)kind_ab << 7) | ((uint32_t)kind_ab << 10) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
+// The MMAs and their commit are called by a whole warp and issued by one
+// elected lane of it: with operands that are the same in every lane, one takes
+// some 20 cycles to issue (from a branch of one lane, 60 to 75).
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(id), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
         : "memory");
 }
 __device__ __forceinline__ void mma_tf32_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
         "r"(a_tmem), "l"(b), "r"(id), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 // 16-byte unit u (0..7) of row r of a 128-byte-swizzled tile
@@ -266,15 +273,17 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
 
     if (warp >= kMmaWarp) {
         // ----------------------------------------------------- MMA issuers
-        const int q = (warp - kMmaWarp) % NQ;
+        // (a uniform role and tile: the MMAs' operands stay in uniform registers)
+        const int role = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0), q = role % NQ;
         const uint32_t t = tmem + q * C::kCols;
         auto wait = [&](uint32_t bar, int parity, int site) {
-            if (!tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site)) return false;
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site)))
+                return false;
             tc::tc_fence_after();
             return true;
         };
-        if (lane == 0 && tiles) {
-            if (warp - kMmaWarp < NQ) {
+        if (tiles) {
+            if (role < NQ) {
                 // scores, into the buffer whose weights, of two tiles before, have been multiplied
                 constexpr uint32_t id = idesc(0, kRows, NT);
                 const uint32_t qb = sb + q * C::kParts * C::kQ;
@@ -288,9 +297,9 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                         for (int k = 0; k < HD / 16; ++k)
                             mma_f16_ss(d, tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
                                        tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id, part || k);
-                    tc::mma_commit(s_full(q, i));
-                    tc::mbar_arrive(s_full(q, i));
-                    tc::mma_commit(k_empty(i & 1));
+                    commit(s_full(q, i));
+                    if (lane == 0) tc::mbar_arrive(s_full(q, i));
+                    commit(k_empty(i & 1));
                 }
             } else {
                 // outputs, OT columns at a time for fp32
@@ -312,13 +321,13 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                                 mma_tf32_ts(d, t + part * C::kOffL + (i & 1) * NT + 8 * k,
                                             tc::sdesc_kmajor_sw128(vb + (k / 4) * HD * 128) + 2 * (k % 4), id,
                                             (!kTwo && i) || part || k);
-                        tc::mma_commit(turn + 1 < kTurns ? t_part : o_done(q, i));
+                        commit(turn + 1 < kTurns ? t_part : o_done(q, i));
                     }
-                    if (ok) tc::mma_commit(v_empty(i & 1));
+                    if (ok) commit(v_empty(i & 1));
                 }
             }
             // every MMA issued has completed before TMEM is released
-            tc::mma_commit(last_bar);
+            commit(last_bar);
             tc::mbar_wait(last_bar, 0, abort_flag, &g_q4_status, 46, false);
         }
     } else if (warp >= NQ * 4) {
@@ -582,23 +591,22 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             float x0, x1;
             unpair(f2_add(l2[0], l2[1]), x0, x1);
             l += x0 + x1;
-            // the outputs up to the tile before are summed; on the new reference
-            if (i) {
-                if constexpr (kTwo) ok = add_tile(i - 1);
-                else ok = wait(o_done(q_of, i - 1), (i - 1) >> 1, 50);
-                if (!ok) break;
-                if (__any_sync(0xffffffffu, move)) {
+            // the outputs up to the tile before, on the new reference
+            if constexpr (kTwo)
+                if (i) ok = add_tile(i - 1);
+            if (ok && i && __any_sync(0xffffffffu, move)) {
+                if constexpr (!kTwo) ok = wait(o_done(q_of, i - 1), (i - 1) >> 1, 50);
 #pragma unroll 1
-                    for (int j = 0; j < HD / 32; ++j) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(tm + C::kOffO + 32 * j, o);
-                        tc::tmem_wait_ld();
+                for (int j = 0; ok && j < HD / 32; ++j) {
+                    uint32_t o[32];
+                    tc::tmem_ld32(tm + C::kOffO + 32 * j, o);
+                    tc::tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                        tc::tmem_st32(tm + C::kOffO + 32 * j, o);
-                    }
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                    tc::tmem_st32(tm + C::kOffO + 32 * j, o);
                 }
             }
+            if (!ok) break;
             tc::tmem_wait_st();
             tc::tc_fence_before();
             tc::mbar_arrive(p_full(q_of, i));
