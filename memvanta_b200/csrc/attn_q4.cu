@@ -16,9 +16,12 @@ namespace mvb {
 
 namespace {
 
-// The sequence of query row r (q_start ascending), by bisection.
-__device__ __forceinline__ int seq_of_row(const AttnQ4Args& a, int64_t r) {
-    if (!a.q_start) return (int)r;
+// The sequence of query row r: r itself, or by bisection of q_start (ascending);
+// -1: none.
+__device__ __forceinline__ int seq_of_row(const AttnQ4Args& a, int r) {
+    if (a.one_seq) return 0;
+    if (!a.q_start) return r;
+    if (r < a.q_start[0] || r >= a.q_start[a.n_seq]) return -1;
     int lo = 0, hi = (int)a.n_seq - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -26,74 +29,6 @@ __device__ __forceinline__ int seq_of_row(const AttnQ4Args& a, int64_t r) {
         else hi = mid - 1;
     }
     return lo;
-}
-
-// One (row, head) per CTA: four warps take every fourth token, lane l holds
-// dimensions (HD / 32) l .. of the running output.
-template <class T, int HD>
-__global__ void __launch_bounds__(128) attn_q4_row_kernel(AttnQ4Args a) {
-    constexpr int E = HD / 32;
-    const int64_t r = blockIdx.x;
-    const int h = blockIdx.y, kvh = h / (int)(a.n_head / a.n_head_kv), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = seq_of_row(a, r);
-    const int64_t ctx = min((int64_t)a.ctx_len[r], (int64_t)min(a.max_ctx, a.max_pages * a.page));
-    const T* q = static_cast<const T*>(a.q) + r * (int64_t)a.q_stride + h * HD;
-    float qv[E], o[E], m = -INFINITY, sum = 0.0f;
-    const int d0 = lane * E, b = d0 / 32;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        qv[i] = to_f32(q[d0 + i]) * a.scale;
-        o[i] = 0.0f;
-    }
-    for (int64_t t = warp; t < ctx; t += 4) {
-        const int64_t pg = a.block_table[(int64_t)s * (int64_t)a.max_pages + t / (int64_t)a.page];
-        if (pg < 0 || pg >= (int64_t)a.n_pages) continue;
-        const int64_t tok = (pg * (int64_t)a.n_head_kv + kvh) * (int64_t)a.page + t % (int64_t)a.page;
-        const uint8_t* kp = a.k_pages + tok * (HD / 2);
-        const uint8_t* vp = a.v_pages + tok * (HD / 2);
-        float kd = bf16_bits_to_f32(a.k_scales[tok * (HD / 32) + b]), vd = bf16_bits_to_f32(a.v_scales[tok * (HD / 32) + b]);
-        float dot = 0.0f, v[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int d = d0 + i, at = (d % 32 / 8 * (HD / 32) + b) * 4 + d % 8 / 2, sh = d % 2 * 4;
-            dot = fmaf(qv[i], (float)((int)((kp[at] >> sh) & 15) - 8) * kd, dot);
-            v[i] = (float)((int)((vp[at] >> sh) & 15) - 8) * vd;
-        }
-        dot = warp_sum(dot);
-        const float mn = fmaxf(m, dot), c = m > -INFINITY ? expf(m - mn) : 0.0f, p = expf(dot - mn);
-        sum = sum * c + p;
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = fmaf(p, v[i], o[i] * c);
-        m = mn;
-    }
-    __shared__ float sm[4], ss[4], so[4][HD];
-#pragma unroll
-    for (int i = 0; i < E; ++i) so[warp][d0 + i] = o[i];
-    if (lane == 0) sm[warp] = m, ss[warp] = sum;
-    __syncthreads();
-    const float mt = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float w[4], den = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = sm[i] > -INFINITY ? expf(sm[i] - mt) : 0.0f;
-        den += ss[i] * w[i];
-    }
-    T* out = static_cast<T*>(a.out) + r * (int64_t)a.out_stride + h * HD;
-    for (int d = threadIdx.x; d < HD; d += 128) {
-        float y = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y = fmaf(w[i], so[i][d], y);
-        out[d] = from_f32<T>(den == 0.0f ? 0.0f : y / den);
-    }
-}
-
-template <class T>
-cudaError_t attn_rows(const AttnQ4Args& a, cudaStream_t s) {
-    const dim3 grid((unsigned)a.n_q, (unsigned)a.n_head);
-    if (a.hd == 64) attn_q4_row_kernel<T, 64><<<grid, 128, 0, s>>>(a);
-    else if (a.hd == 128) attn_q4_row_kernel<T, 128><<<grid, 128, 0, s>>>(a);
-    else attn_q4_row_kernel<T, 256><<<grid, 128, 0, s>>>(a);
-    return cudaGetLastError();
 }
 
 // ------------------------------------------------------------- primitives
@@ -153,8 +88,8 @@ __device__ __forceinline__ void mma1688(float (&d)[4], const float (&a)[4], floa
 // four heads (PACK: rows 4..7 repeat heads 0..3, so a lane's weights are
 // already there) and a second MMA for more.  The tensor core ignores the low
 // 13 bits of a tf32 operand, so the first part needs no masking; half-precision
-// queries' weights go in as one part, and p carries a factor 1 + 2^-12 that
-// makes up for what that cut takes off on average.
+// queries' weights go in as one part, and p carries a factor kCut that makes up
+// for what that cut takes off on average.
 constexpr int kWarps = 4, kStages = 3;
 
 template <int HD>
@@ -325,8 +260,9 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     uint32_t head_slot;
     const uint32_t page = (uint32_t)a.page, page_rows = (uint32_t)H * page;
     auto new_unit = [&] {
-        table = a.block_table + (int64_t)ahead.row * (int64_t)a.max_pages;
-        ctx = min(a.ctx_len[ahead.row], (int)a.max_ctx);
+        const int seq = seq_of_row(a, ahead.row);
+        table = a.block_table + (int64_t)max(seq, 0) * (int64_t)a.max_pages;
+        ctx = seq < 0 ? 0 : min(a.ctx_len[ahead.row], (int)a.max_ctx);
         head_slot = (uint32_t)ahead.kvh * page;
     };
     auto look_up = [&] {
@@ -531,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
                 for (int i = 0; i < 2; ++i) {
                     p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
                     l_run += p[i];
-                    if constexpr (!kTwo) p[i] *= 1.000244140625f;
+                    if constexpr (!kTwo) p[i] *= kCut;
                     load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
                 }
                 const uint64_t pp = pair(p[0], p[1]);
@@ -704,8 +640,9 @@ uint64_t resident_ctas(const void* kernel, int threads, int smem) {
     return (uint64_t)std::max(1, per * sms);
 }
 
+// `need`: only says how much scratch the launch takes.
 template <class T, int HD, bool PACK>
-cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
+cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     using X = Q4Tile<HD>;
     constexpr int kHeads = PACK ? 4 : 8;
     const int smem = kWarps * X::kRing + kWarps * kStages * 8;
@@ -727,10 +664,16 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     const uint64_t grid = std::max<uint64_t>(1, std::min<uint64_t>(slots, most)), warps = grid * kWarps;
     sp.by_unit = units <= warps;
     const uint64_t joins = sp.by_unit ? units : warps;
-    keep_pool_memory();
     const uint64_t parts = 2 * warps * sp.heads * (HD + 2) * 4;
-    uint8_t* scratch = nullptr;
-    if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), parts + joins * sizeof(int4), s)) return e;
+    if (need) {
+        *need = parts + joins * sizeof(int4);
+        return cudaSuccess;
+    }
+    uint8_t* scratch = static_cast<uint8_t*>(a.workspace);
+    if (!scratch) {
+        keep_pool_memory();
+        if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), parts + joins * sizeof(int4), s)) return e;
+    }
     sp.scratch = reinterpret_cast<float*>(scratch);
     sp.joins = reinterpret_cast<int4*>(scratch + parts);
     // many parts a unit: all 1024 threads; few: as many groups as there are parts, at most
@@ -741,31 +684,51 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess)
         e = launch_pdl(attn_q4_join_kernel<T, HD>, join_grid, dim3(join_threads), 0, s, a, sp, (int64_t)warps);
-    cudaFreeAsync(scratch, s);
+    if (!a.workspace) cudaFreeAsync(scratch, s);
     return e;
 }
 template <class T>
-cudaError_t attn_decode(const AttnQ4Args& a, cudaStream_t s) {
+cudaError_t attn_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     if constexpr (sizeof(T) == 4) {
         if (a.n_head / a.n_head_kv <= 4) {
-            if (a.hd == 64) return launch_decode<T, 64, true>(a, s);
-            if (a.hd == 128) return launch_decode<T, 128, true>(a, s);
-            return launch_decode<T, 256, true>(a, s);
+            if (a.hd == 64) return launch_decode<T, 64, true>(a, s, need);
+            if (a.hd == 128) return launch_decode<T, 128, true>(a, s, need);
+            return launch_decode<T, 256, true>(a, s, need);
         }
     }
-    if (a.hd == 64) return launch_decode<T, 64, false>(a, s);
-    if (a.hd == 128) return launch_decode<T, 128, false>(a, s);
-    return launch_decode<T, 256, false>(a, s);
+    if (a.hd == 64) return launch_decode<T, 64, false>(a, s, need);
+    if (a.hd == 128) return launch_decode<T, 128, false>(a, s, need);
+    return launch_decode<T, 256, false>(a, s, need);
+}
+cudaError_t decode_of(int type, const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
+    if (type == kTypeF32) return attn_decode<float>(a, s, need);
+    if (type == kTypeF16) return attn_decode<__half>(a, s, need);
+    return attn_decode<__nv_bfloat16>(a, s, need);
+}
+
+// Chunks go row by row through the kernel above while they are small: a row and
+// kv head costs it 54 ps a token (head_dim 128: 57 us for 131,071 tokens of 8),
+// whereas a wave of the tensor-core kernel's CTAs takes 19 ns a token (fp32
+// queries 28 ns) however few of its 128 rows are used -- 350 or 520 times that.
+bool rows_one_by_one(int type, const AttnQ4Args& a) {
+    const uint64_t G = a.n_head / a.n_head_kv, heads = type == kTypeF32 && G <= 4 ? 4 : 8;
+    const uint64_t rpt = 128 / std::min<uint64_t>(G, 128);
+    const uint64_t ctas = a.n_seq * a.n_head_kv * ((G + 127) / 128) * ((a.max_q + rpt - 1) / rpt);
+    return a.n_q * a.n_head_kv * ((G + heads - 1) / heads) < (type == kTypeF32 ? 520 : 350) * ((ctas + 147) / 148);
 }
 
 }  // namespace
 
+uint64_t attn_q4_workspace(int type, const AttnQ4Args& a) {
+    uint64_t need = 0;
+    decode_of(type, a, nullptr, &need);
+    return need;
+}
+
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s) {
     if (!a.n_q || !a.n_head) return cudaSuccess;
-    if (a.q_start) return attn_q4_prefill(type, a, s);
-    if (type == kTypeF32) return attn_decode<float>(a, s);
-    if (type == kTypeF16) return attn_decode<__half>(a, s);
-    return attn_decode<__nv_bfloat16>(a, s);
+    if ((a.q_start || a.one_seq) && !rows_one_by_one(type, a)) return attn_q4_prefill(type, a, s);
+    return decode_of(type, a, s, nullptr);
 }
 
 }  // namespace mvb

@@ -56,12 +56,10 @@ cudaError_t q4_status_take(int* status) {
 namespace {
 
 constexpr int kRows = 128;  // of a query tile: TMEM lanes
-// Half-precision queries: factor on the weights for what their cut to 11 bits
-// takes off on average, 1 + 2^-11 / (2 ln 2), and its logarithm.
 // fp32: factor on the outputs for the 16 cut sums of a token tile's MMAs
 // (measured: they come out 1.0e-6 short, of 1.2e-6 in all).
 constexpr float kSumCut = 1.0f + 1.0f / 1048576;
-constexpr float kCut = 1.00035225f, kCutLog2 = 5.0811e-4f;
+constexpr float kCutLog2 = 5.0811e-4f;  // log2(kCut)
 constexpr int kRing = 4;    // tiles whose exponent and token masks are kept
 
 template <int HD, int NQ, bool TWO>
@@ -156,10 +154,21 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
     const int chunk = rest % p.chunks;
     rest /= p.chunks;
     const int kvh = rest % H, seq = rest / H;
-    const int64_t seq0 = min(max(a.q_start[seq], 0), (int)a.n_q), seq1 = min(max(a.q_start[seq + 1], 0), (int)a.n_q);
+    const int64_t seq0 = a.one_seq ? 0 : min(max(a.q_start[seq], 0), (int)a.n_q);
+    const int64_t seq1 = a.one_seq ? (int64_t)a.n_q : min(max(a.q_start[seq + 1], 0), (int)a.n_q);
     const int64_t row0 = seq0 + (int64_t)qt * NQ * p.rpt;
-    if (row0 >= seq1) return;
     const int h0 = kvh * G + chunk * p.heads, nh = min(p.heads, G - chunk * p.heads);
+    if (qt == p.q_tiles - 1) {  // rows of no chunk, and past max_q, are zeros
+        auto zeros = [&](int64_t from, int64_t to) {
+            for (int64_t r = from; r < to; ++r)
+                for (int k = threadIdx.x; k < nh * HD; k += blockDim.x)
+                    static_cast<T*>(a.out)[r * (int64_t)a.out_stride + (int64_t)h0 * HD + k] = T(0.0f);
+        };
+        zeros(seq0 + (int64_t)p.q_tiles * NQ * p.rpt, seq1);
+        if (seq == 0) zeros(0, seq0);
+        if (seq == (int)a.n_seq - 1) zeros(max(seq0, seq1), (int64_t)a.n_q);
+    }
+    if (row0 >= seq1) return;
 
     const uint32_t bars = sb + C::kOffBar;
     auto k_full = [&](int s) { return bars + 8 * s; };

@@ -626,7 +626,7 @@ MV_API int mv_paged_attn_q4(int type, const void* q, uint64_t q_row_stride, uint
         return fail(MV_ERR_INVALID, "the pool holds 2^32 or more (token, kv head) rows");
     mvb::AttnQ4Args a{q, q_row_stride, n_seq, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
                       static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
-                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, nullptr, 1,
+                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, nullptr, 0, 1,
                       ctx_len, std::min(max_ctx, max_pages * page),
                       scale > 0.0f ? scale : 1.0f / std::sqrt((float)hd), out, out_row_stride};
     CK(mvb::attn_q4(type, a, as_stream(stream)));
@@ -651,7 +651,7 @@ MV_API int mv_paged_attn_q4_prefill(int type, const void* q, uint64_t q_row_stri
     if (!q_start || !max_q || max_q > n_q) return fail(MV_ERR_INVALID, "prefill needs q_start and max_q in 1..n_q");
     mvb::AttnQ4Args a{q, q_row_stride, n_q, n_head, n_head_kv, hd, static_cast<const uint8_t*>(k_pages),
                       static_cast<const uint8_t*>(v_pages), static_cast<const uint16_t*>(k_scales),
-                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, q_start,
+                      static_cast<const uint16_t*>(v_scales), block_table, n_seq, max_pages, page, n_pages, q_start, 0,
                       max_q, ctx_len, std::min(max_ctx, max_pages * page),
                       scale > 0.0f ? scale : 1.0f / std::sqrt((float)hd), out, out_row_stride};
     CK(mvb::attn_q4(type, a, as_stream(stream)));

@@ -189,6 +189,7 @@ struct KvRows {  // cache rows by sequence and position
     const int32_t* pos;
     const int32_t* block_table;  // [n_seq][max_pages]
     uint64_t n_seq, max_pages, page, n_pages;
+    int row_is_seq = 0;  // 1: row r is sequence r
 };
 struct RopeAppendArgs {
     int kv_type;
@@ -207,7 +208,8 @@ struct RopeAppendArgs {
     void* v_pages;
     void* k_scales;
     void* v_scales;
-    int q_parts = 0;  // set by rope_kv_append
+    int32_t* ctx_out = nullptr;  // optional: receives pos + 1 per row
+    int q_parts = 0;             // set by rope_kv_append
 };
 cudaError_t rope_kv_append(int type, const RopeAppendArgs& a, cudaStream_t s);
 struct KvReadArgs {
@@ -232,15 +234,19 @@ struct AttnQ4Args {
     const int32_t* block_table;  // [n_seq][max_pages]
     uint64_t n_seq, max_pages, page, n_pages;
     const int32_t* q_start;  // [n_seq + 1] first row of each sequence; nullptr: row r is sequence r
+    int one_seq;             // 1: all rows are sequence 0's (q_start unused)
     uint64_t max_q;          // most rows of one sequence
     const int32_t* ctx_len;  // per row
     uint64_t max_ctx;
     float scale;
     void* out;
     uint64_t out_stride;
+    void* workspace = nullptr;  // attn_q4_workspace bytes; nullptr: stream-ordered scratch
 };
+// Scratch of one query row per sequence, for any context up to max_ctx.
+uint64_t attn_q4_workspace(int type, const AttnQ4Args& a);
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s);
-// attn_q4_prefill.cu : the same for a.q_start's chunks, on tcgen05
+// attn_q4_prefill.cu : the same for chunks (q_start, one_seq), on tcgen05
 cudaError_t attn_q4_prefill(int type, const AttnQ4Args& a, cudaStream_t s);
 cudaError_t q4_status_take(int* status);
 

@@ -171,7 +171,7 @@ __device__ __forceinline__ void rotated8(const T* __restrict__ x, int d, int rot
 // page that does not exist.
 __device__ __forceinline__ int64_t kv_slot_page(const KvRows& k, int64_t r, int* slot) {
     const int p = k.pos[r];
-    const int s = k.seq ? k.seq[r] : 0;
+    const int s = k.row_is_seq ? (int)r : k.seq ? k.seq[r] : 0;
     if (p < 0 || (uint64_t)p >= k.max_pages * k.page || s < 0 || (uint64_t)s >= k.n_seq) return -1;
     const int64_t pg = k.block_table[(int64_t)s * (int64_t)k.max_pages + p / (int)k.page];
     *slot = p % (int)k.page;
@@ -181,6 +181,7 @@ __device__ __forceinline__ int64_t kv_slot_page(const KvRows& k, int64_t r, int*
 template <class T, bool VEC, int KVT>
 __global__ void __launch_bounds__(256) rope_kv_append_kernel(RopeAppendArgs a) {
     const int64_t r = blockIdx.x;
+    if (a.ctx_out && blockIdx.y == 0 && threadIdx.x == 0) a.ctx_out[r] = a.rows.pos[r] + 1;
     if ((int)blockIdx.y < a.q_parts) {
         rope_row<T, VEC ? 16 / (int)sizeof(T) : 1, VEC>(a.q, r, blockIdx.y, a.q_parts);
         return;

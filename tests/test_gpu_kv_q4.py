@@ -532,6 +532,113 @@ def test_prefill_rows_of_any_length(cuda):
     assert not got[torch.from_numpy(ctx == 0).cuda()].any()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,H,hd,page,chunks", [
+    (8, 8, 64, 16, [(40, 100), (1, 3), (0, 0), (29, 0), (300, 7)]),
+    (12, 4, 128, 13, [(200, 0), (30, 500), (127, 1)]),
+    (10, 5, 128, 64, [(129, 130)]),
+    (7, 7, 256, 1, [(90, 60), (64, 0)]),
+    (12, 6, 256, 128, [(260, 1)]),
+    (130, 1, 64, 32, [(70, 70)]),
+    (33, 3, 64, 7, [(200, 1)])])
+def test_prefill_of_many_rows(cuda, heads, H, hd, page, chunks, dtype):
+    """Chunks large enough for the tensor-core kernel in every type and head_dim,
+    with groups that leave tile rows over and that take more than one tile."""
+    import torch
+    starts = np.concatenate([[0], np.cumsum([n for n, _ in chunks])]).astype(np.int32)
+    ctx = np.concatenate([np.arange(p + 1, p + n + 1) for n, p in chunks]).astype(np.int32)
+    seq = np.concatenate([[i] * n for i, (n, _) in enumerate(chunks)]).astype(int)
+    t, total = scattered([n + p for n, p in chunks], page, 61)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 62)
+    q = randn((len(ctx), heads, hd), 63, dtype, 1.3)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    args = (q, kp, vp, ks, vs, dev(t), dev(starts), max(n for n, _ in chunks), dev(ctx), int(ctx.max()))
+    got = mv.paged_attn_q4_prefill(*args)
+    want, bound = attention64(q, kp, ks, vp, vs, t, seq, ctx, page, hd ** -0.5)
+    check_attention(got, want, bound)
+    assert torch.equal(got, mv.paged_attn_q4_prefill(*args))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("hd,H,heads", [(64, 8, 16), (128, 8, 8), (256, 8, 8)])
+def test_prefill_of_many_rows_of_any_length(cuda, hd, H, heads, dtype):
+    """No order among the rows' lengths, rows of no token among them, a table
+    with pages that are missing (their tokens do not count), rows past the last
+    chunk and rows before the first (zeros)."""
+    import torch
+    page, T, rows = 16, 300, 150
+    rng = np.random.default_rng(64)
+    ctx = rng.choice([0, 0, 1, 2, 63, 64, 65, 127, 128, 129, 255, T - 1, T], size=rows).astype(np.int32)
+    ctx[:3] = 0, T, 1
+    t, total = scattered([T], page, 65)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 66)
+    q = randn((rows, heads, hd), 67, dtype)
+    holes = t.copy()
+    holes[0, [1, 7, 8, 18]] = [-1, 2 ** 31 - 1, total, -2 ** 31]
+    starts = np.array([4, rows - 5], np.int32)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(holes), dev(starts), rows, dev(ctx), T)
+    # the tokens of the pages that are there, as a cache of their own
+    there = np.array([p for p in range(-(-T // page)) if p not in (1, 7, 8, 18)])
+    inside = np.array([sum(min(page, max(0, c - page * p)) for p in there) for c in ctx])
+    want, bound = attention64(q, kp, ks, vp, vs, t[:, there], [0] * rows, inside, page, hd ** -0.5)
+    used = np.zeros(rows, bool)
+    used[4:rows - 5] = True
+    keep = torch.from_numpy(used & (inside > 0)).cuda()
+    check_attention(got[keep], want[keep], bound[keep])
+    assert not got[~keep].any()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_prefill_of_many_rows_with_garbage_past_the_context(cuda, dtype):
+    """NaN and infinite scales in the tokens that a row does not reach leave it
+    as it is, inside its tile and in the pages after; a row that reaches a value
+    block of NaN has NaN in that block's dimensions."""
+    import torch
+    hd, H, heads, page, T, cut = 128, 8, 8, 16, 256, 150
+    ctx = np.arange(T - 120 + 1, T + 1, dtype=np.int32)  # 137 .. 256
+    t, total = scattered([T], page, 68)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 69)
+    q = randn((len(ctx), heads, hd), 70, dtype)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    args = (dev(t), dev(np.array([0, len(ctx)], np.int32)), len(ctx), dev(ctx), T)
+    want, bound = attention64(q, kp, ks, vp, vs, t, [0] * len(ctx), ctx, page, hd ** -0.5)
+    # token `cut` and all later ones
+    for token in range(cut, T):
+        pg, o = int(t[0, token // page]), token % page
+        vs[pg, :, o, 1] = float("nan")
+        if token > cut:
+            ks[pg, :, o] = float("nan") if token % 2 else float("inf")
+            vs[pg, :, o] = float("inf") if token % 3 else float("nan")
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, *args)
+    clean = torch.from_numpy(ctx <= cut).cuda()
+    check_attention(got[clean], want[clean], bound[clean])
+    one = got[torch.from_numpy(ctx == cut + 1).cuda()][0]
+    assert one[:, 32:64].isnan().all()
+    rest = torch.cat([one[:, :32], one[:, 64:]], -1)
+    row = int(np.flatnonzero(ctx == cut + 1)[0])
+    w, b = (torch.cat([x[row][:, :32], x[row][:, 64:]], -1) for x in (want, bound))
+    check_attention(rest[None], w[None], b[None])
+    assert got[torch.from_numpy(ctx > cut + 1).cuda()].isnan().all()
+
+
+def test_large_and_small_chunks_agree(cuda):
+    """The same rows as one large chunk, in small ones, and one by one."""
+    import torch
+    hd, H, heads, page, T = 128, 8, 32, 32, 400
+    ctx = np.arange(T - 100 + 1, T + 1, dtype=np.int32)
+    t, total = scattered([T], page, 71)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 72)
+    q = randn((100, heads, hd), 73)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    want, bound = attention64(q, kp, ks, vp, vs, t, [0] * 100, ctx, page, hd ** -0.5)
+    for n in (100, 10, 1):
+        got = torch.cat([mv.paged_attn_q4_prefill(q[i:i + n], kp, vp, ks, vs, dev(t),
+                                                  dev(np.array([0, n], np.int32)), n, dev(ctx[i:i + n]), T)
+                         for i in range(0, 100, n)])
+        check_attention(got, want, bound)
+
+
 # ----------------------------------------------------------------- refusals
 
 def test_refusals(cuda):
