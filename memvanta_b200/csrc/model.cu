@@ -339,6 +339,7 @@ struct mv_model_s {
     float eps = 1e-5f, theta = 10000.0f;
     uint64_t hd = 0, kv_dim = 0, page = 128, n_pages = 0;
     int kv_type = MV_KV_F16;
+    uint8_t* q4_workspace = nullptr;  // scratch of the decode step's attention over a 4-bit cache
     uint64_t pos = 0;
 
     std::vector<mv_weight_s*> owned;  // every uploaded weight
@@ -719,6 +720,24 @@ void project_decode(mv_model_s* m, mv_weight_s* w, const float* x, const float* 
 // every row is a token of the one sequence whose pages row 0 lists).
 void rope_append(mv_model_s* m, const mvb::Layer& L, float* qkv, uint64_t rows, const int32_t* pos, int32_t* ctx_out,
                  bool plain = false, const int32_t* table = nullptr, int table_ld = 0) {
+    if (m->kv_type == MV_KV_Q4_0) {
+        const uint64_t pages = table ? (uint64_t)table_ld : m->n_pages;
+        mvb::RopeAppendArgs a{};
+        a.kv_type = MV_KV_Q4_0;
+        a.q = {qkv, m->qkvw, m->hd, qkv, m->qkvw, m->hd, m->nh, m->hd, m->hd, MV_ROPE_HALF,
+               m->rope_cos, m->rope_sin, m->n_ctx, pos};
+        a.k = qkv + m->nh * m->hd, a.v = qkv + m->nh * m->hd + m->kvd;
+        a.k_stride = a.v_stride = m->qkvw, a.k_head_stride = a.v_head_stride = m->hd;
+        a.n_head_kv = m->nkv, a.hd = a.rot = m->hd, a.layout = MV_ROPE_HALF;
+        a.cos_t = m->rope_cos, a.sin_t = m->rope_sin, a.n_pos = m->n_ctx, a.n_rows = rows;
+        // rows of the one sequence (the identity table), or a row of each sequence of a set
+        a.rows = {nullptr, pos, table ? table : m->table, table ? rows : 1, pages, m->page,
+                  table ? rows * pages : m->n_pages, table != nullptr};
+        a.k_pages = L.k_pages, a.v_pages = L.v_pages, a.k_scales = L.k_scales, a.v_scales = L.v_scales;
+        a.ctx_out = ctx_out;
+        ck(mvb::rope_kv_append(MV_TYPE_F32, a, m->stream), "rope_append");
+        return;
+    }
     if (!table) table = m->table;
     const uint64_t QKVW = m->qkvw;  // this rank's heads
     cudaError_t e;
@@ -746,6 +765,20 @@ mvb::AttnArgs attn_args(mv_model_s* m, const mvb::Layer& L, const float* q, uint
                         const int32_t* ctx, uint64_t max_ctx, float* out) {
     return mvb::AttnArgs{m->kv_type, q, q_stride, n_q, m->nh, m->nkv, m->hd, L.k_pages, L.v_pages,
                          L.k_scales, L.v_scales, m->table, m->n_pages, m->page, ctx, max_ctx, out};
+}
+
+// Attention over a 4-bit cache: `rows` query rows of the one sequence, or with
+// a set's table a row of each of its sequences.
+void attention_q4(mv_model_s* m, const mvb::Layer& L, const float* qkv, uint64_t rows, const int32_t* ctx,
+                  uint64_t max_ctx, float* out, const int32_t* table = nullptr, uint64_t pages = 0,
+                  void* workspace = nullptr) {
+    mvb::AttnQ4Args a{qkv, m->qkvw, rows, m->nh, m->nkv, m->hd, L.k_pages, L.v_pages,
+                      reinterpret_cast<const uint16_t*>(L.k_scales), reinterpret_cast<const uint16_t*>(L.v_scales),
+                      table ? table : m->table, table ? rows : 1, table ? pages : m->n_pages, m->page,
+                      table ? rows * pages : m->n_pages, nullptr, table ? 0 : 1, rows, ctx, max_ctx,
+                      1.0f / std::sqrt((float)m->hd), out, m->nh * m->hd};
+    a.workspace = workspace;
+    ck(mvb::attn_q4(MV_TYPE_F32, a, m->stream), "attention (4-bit cache)");
 }
 
 // Sync points of one step under tensor parallelism (tp.cuh): per layer the
@@ -840,8 +873,12 @@ void launch_decode(mv_model_s* m, bool with_logits) {
         } else {
             rope_append(m, L, m->qkv, 1, m->pos_dev, m->ctx_dev);
             float* out = tp ? m->ATT_l : m->att;
-            const mvb::AttnArgs aa = attn_args(m, L, m->qkv, m->qkvw, 1, m->ctx_dev, m->n_ctx, out);
-            ck(m->attn_split ? mvb::paged_attn_decode_split(aa, s) : mvb::paged_attn_decode(aa, s), "attention");
+            if (m->kv_type == MV_KV_Q4_0) {
+                attention_q4(m, L, m->qkv, 1, m->ctx_dev, m->n_ctx, out, nullptr, 0, m->q4_workspace);
+            } else {
+                const mvb::AttnArgs aa = attn_args(m, L, m->qkv, m->qkvw, 1, m->ctx_dev, m->n_ctx, out);
+                ck(m->attn_split ? mvb::paged_attn_decode_split(aa, s) : mvb::paged_attn_decode(aa, s), "attention");
+            }
             if (tp) ck(mvb::tp_scatter_ll(m->tp, out, m->Dl, m->off_att, r * m->Dl, pt_att(l), s), "scatter");
         }
         if (tp) {
@@ -1010,6 +1047,11 @@ void setup_persistent_decode(mv_model_s* m) {
     m->mk = true;
 }
 
+// Scales of a cached token row in units of 4 bytes (Q4_0: two bf16).
+uint64_t scale_floats(int kv_type, uint64_t kvd) {
+    return mvb::kv_row_scales(kv_type, kvd) / (kv_type == MV_KV_Q4_0 ? 2 : 1);
+}
+
 void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, int kv_type, int rank = 0,
                 int world = 1, uint64_t tp_bmax = 0) {
     mvb::GgufReader f(path);
@@ -1043,7 +1085,8 @@ void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, in
     if (m->hd != 64 && m->hd != 128 && m->hd != 256)
         throw ModelError(MV_ERR_UNSUPPORTED, "device attention supports head_dim 64, 128, 256");
     if (m->n_head / m->n_head_kv > 8) throw ModelError(MV_ERR_UNSUPPORTED, "GQA group above 8");
-    if (kv_type < 0 || kv_type > 3) throw ModelError(MV_ERR_UNSUPPORTED, "unknown KV cache type");
+    if (kv_type < 0 || kv_type > 4) throw ModelError(MV_ERR_UNSUPPORTED, "unknown KV cache type");
+    if (world > 1 && kv_type == MV_KV_Q4_0) throw ModelError(MV_ERR_UNSUPPORTED, "the Q4_0 cache runs on one GPU");
     if (kv_type == MV_KV_Q8_0 && m->kv_dim % 32) throw ModelError(MV_ERR_INVALID, "Q8_0 KV needs kv_dim % 32 == 0");
     if (world > 1 && kv_type == MV_KV_Q8)
         throw ModelError(MV_ERR_UNSUPPORTED, "tensor parallelism splits the kv heads; the Q8 cache's per-token scale "
@@ -1077,7 +1120,7 @@ void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, in
     else m->output = upload_rows(m, up, f, {{out ? out : &te, rank * m->Vl, m->Vl}}, false);
 
     const uint64_t rows = m->n_pages * m->page;
-    const uint64_t rb = mvb::kv_row_bytes(kv_type, m->kvd), ns = mvb::kv_row_scales(kv_type, m->kvd);
+    const uint64_t rb = mvb::kv_row_bytes(kv_type, m->kvd), ns = scale_floats(kv_type, m->kvd);
     m->layers.resize(m->n_layer);
     for (uint64_t i = 0; i < m->n_layer; ++i) {
         auto name = [&](const char* s) { return "blk." + std::to_string(i) + s; };
@@ -1168,6 +1211,11 @@ void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, in
     m->history = dalloc<int32_t>(m, m->n_ctx + 1);
     ck(cudaMallocHost(reinterpret_cast<void**>(&m->logits_host), m->vocab * sizeof(float)), "cudaMallocHost");
     ensure_prefill(m, 1);  // identity block table
+    if (kv_type == MV_KV_Q4_0) {
+        mvb::AttnQ4Args a{};
+        a.n_q = 1, a.n_head = m->nh, a.n_head_kv = m->nkv, a.hd = m->hd, a.page = m->page, a.max_ctx = m->n_ctx;
+        m->q4_workspace = dalloc<uint8_t>(m, mvb::attn_q4_workspace(MV_TYPE_F32, a));
+    }
     {
         const char* env = std::getenv("MV_ATTN_SPLIT");
         m->attn_split = env && std::string(env) == "1";
@@ -1367,8 +1415,11 @@ void prefill_chunk(mv_model_s* m, uint64_t off, uint64_t B, bool logits_last, co
                                      tp ? m->ATT_l : m->ATT);
         // single GPU, tensor-core o projection: the attention kernel also
         // writes the o GEMM's Q8 input (no separate quantisation launch)
-        const bool fuse_o = !tp && !st && B >= 2 && L.o->type == 2;
-        if (st) {
+        const bool fuse_o = !tp && !st && B >= 2 && L.o->type == 2 && m->kv_type != MV_KV_Q4_0;
+        if (m->kv_type == MV_KV_Q4_0) {
+            attention_q4(m, L, m->QKV, B, ctx, st ? st->max_ctx : start + B, m->ATT, st ? st->table : nullptr,
+                         st ? st->pages : 0);
+        } else if (st) {
             aa.block_table = st->table;
             aa.max_pages = st->pages;
             ck(m->attn_split ? mvb::paged_attn_decode_split(aa, s) : mvb::paged_attn_decode(aa, s), "attention");
@@ -1564,7 +1615,7 @@ MV_API uint64_t mv_model_kv_bytes(mv_model_t m) {
     if (!m) return 0;
     const uint64_t pages = (m->pos + m->page - 1) / m->page;
     const uint64_t per_row = mvb::kv_row_bytes(m->kv_type, m->kvd) +  // this rank's kv heads
-                             4 * mvb::kv_row_scales(m->kv_type, m->kvd);
+                             4 * scale_floats(m->kv_type, m->kvd);
     return 2 * m->n_layer * pages * m->page * per_row;
 }
 
@@ -1754,7 +1805,7 @@ void seqs_open(mv_model_s* m, mv_seqs_s* S, uint64_t n_seq, uint64_t ctx) {
     S->slot.resize(n_seq);
     for (uint64_t i = 0; i < n_seq; ++i) S->slot[i] = n_seq - 1 - i;
     const uint64_t rows = n_seq * S->pages * m->page;
-    const uint64_t rb = mvb::kv_row_bytes(m->kv_type, m->kvd), ns = mvb::kv_row_scales(m->kv_type, m->kvd);
+    const uint64_t rb = mvb::kv_row_bytes(m->kv_type, m->kvd), ns = scale_floats(m->kv_type, m->kvd);
     S->pool = m->layers;
     for (auto& L : S->pool) {
         L.k_pages = S->alloc<uint8_t>(rows * rb);
