@@ -42,7 +42,8 @@ __device__ __forceinline__ void cp_async_fill(uint32_t dst, const void* src, int
     if constexpr (N == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes)
+                     : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -338,7 +339,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         // this warp's part of the unit: stages at.stage .. end - 1
         const int from = at.stage, end = min(at.stages, from + count - n), start = n;
         const int h0 = at.kvh * G + at.chunk * sp.heads, nh = min(sp.heads, G - at.chunk * sp.heads);
-        const T* q = static_cast<const T*>(a.q) + (int64_t)at.row * (int64_t)a.q_stride + (int64_t)(h0 + min(hrow, nh - 1)) * HD;
+        const T* q = static_cast<const T*>(a.q) + (int64_t)at.row * (int64_t)a.q_stride +
+                     (int64_t)(h0 + min(hrow, nh - 1)) * HD;
         float x[NB][8], mx = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -445,7 +447,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
             if (__any_sync(0xffffffffu, mx > m_run + 8.0f)) {
                 const float m_new = fmaxf(m_run, mx), alpha = m_new == -INFINITY ? 0.0f : ex2(m_run - m_new);
                 l_run *= alpha;
-                const uint64_t aa = pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
+                const uint64_t aa =
+                pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -525,7 +528,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         float* dst = whole ? nullptr : sp.scratch + part * sp.heads * HD;
         T* out = static_cast<T*>(a.out) + (int64_t)at.row * (int64_t)a.out_stride + (int64_t)h0 * HD;
         if (!whole && t == 0 && g < nh)
-            *reinterpret_cast<float2*>(sp.scratch + ((int64_t)gridDim.x * kWarps * 2 * HD + part * 2) * sp.heads + 2 * g) = make_float2(m_run, l);
+            *reinterpret_cast<float2*>(sp.scratch + ((int64_t)gridDim.x * kWarps * 2 * HD + part * 2) * sp.heads + 2 * g) =
+                make_float2(m_run, l);
         // sums of the two heads of this lane's columns
         float inv[2];
 #pragma unroll
@@ -672,13 +676,15 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     uint8_t* scratch = static_cast<uint8_t*>(a.workspace);
     if (!scratch) {
         keep_pool_memory();
-        if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), parts + joins * sizeof(int4), s)) return e;
+        const uint64_t bytes = parts + joins * sizeof(int4);
+        if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), bytes, s)) return e;
     }
     sp.scratch = reinterpret_cast<float*>(scratch);
     sp.joins = reinterpret_cast<int4*>(scratch + parts);
     // many parts a unit: all 1024 threads; few: as many groups as there are parts, at most
     const uint64_t unit_parts = std::min(warps, most) / std::max<uint64_t>(1, std::min(units, warps)) + 2;
-    const unsigned join_threads = (unsigned)std::min<uint64_t>(kJoin, std::max<uint64_t>(128, (unit_parts * (HD / 4) + 127) / 128 * 128));
+    const unsigned join_threads =
+        (unsigned)std::min<uint64_t>(kJoin, std::max<uint64_t>(128, (unit_parts * (HD / 4) + 127) / 128 * 128));
     const dim3 join_grid((unsigned)joins, sp.by_unit ? (unsigned)sp.heads : 1u, 1u);
     kernel<<<(unsigned)grid, kWarps * 32, smem, s>>>(a, sp);
     cudaError_t e = cudaGetLastError();

@@ -209,7 +209,6 @@ struct RopeAppendArgs {
     void* k_scales;
     void* v_scales;
     int32_t* ctx_out = nullptr;  // optional: receives pos + 1 per row
-    int q_parts = 0;             // set by rope_kv_append
 };
 cudaError_t rope_kv_append(int type, const RopeAppendArgs& a, cudaStream_t s);
 struct KvReadArgs {

@@ -23,6 +23,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -45,85 +46,172 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements <-> fp32 registers; VEC: the address is aligned for
-// 16-byte accesses (32-bit types: two of them for N = 8).
+// N consecutive elements, held as loaded (half types in half the registers)
+// until they are used.  VEC: the address is aligned for 16-byte accesses.
+template <class T, int N, bool VEC>
+struct Held {
+    static constexpr int kBytes = N * (int)sizeof(T), kWords = kBytes / 4;
+    static constexpr bool kWide = VEC && kBytes % 16 == 0;
+    uint32_t w[kWide ? kWords : 1];
+    T v[kWide ? 1 : N];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+                w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) =
+                    make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = v[i];
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[N]) const {
+        if constexpr (kWide && sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = __uint_as_float(w[i]);
+        } else if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const uint16_t lo = (uint16_t)(w[i] & 0xffffu), hi = (uint16_t)(w[i] >> 16);
+                x[2 * i] = to_f32(reinterpret_cast<const T&>(lo));
+                x[2 * i + 1] = to_f32(reinterpret_cast<const T&>(hi));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = to_f32(v[i]);
+        }
+    }
+    __device__ __forceinline__ void set(const float (&x)[N]) {
+        if constexpr (kWide && sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = __float_as_uint(x[i]);
+        } else if constexpr (kWide && std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = reinterpret_cast<const uint32_t&>(h);
+            }
+        } else if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = reinterpret_cast<const uint32_t&>(h);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = from_f32<T>(x[i]);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+        const float none[N] = {};
+        set(none);
+    }
+};
 template <int N, bool VEC, class T>
 __device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
-    if constexpr (VEC && sizeof(T) == 4 && N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + i);
-            x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-        }
-    } else if constexpr (VEC && sizeof(T) == 2 && N == 8) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint16_t lo = (uint16_t)(w[i] & 0xffffu), hi = (uint16_t)(w[i] >> 16);
-            x[2 * i] = to_f32(reinterpret_cast<const T&>(lo));
-            x[2 * i + 1] = to_f32(reinterpret_cast<const T&>(hi));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_f32(p[i]);
-    }
+    Held<T, N, VEC> h;
+    h.load(p);
+    h.get(x);
 }
 template <int N, bool VEC, class T>
 __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
-    if constexpr (VEC && sizeof(T) == 4 && N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-    } else if constexpr (VEC && sizeof(T) == 2 && N == 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const T a = from_f32<T>(x[2 * i]), b = from_f32<T>(x[2 * i + 1]);
-            w[i] = (uint32_t)reinterpret_cast<const uint16_t&>(a) |
-                   ((uint32_t)reinterpret_cast<const uint16_t&>(b) << 16);
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = from_f32<T>(x[i]);
-    }
+    Held<T, N, VEC> h;
+    h.set(x);
+    h.store(p);
+}
+
+// Two floats in a register pair, and the instructions on both (each rounded as
+// the single one).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
 // Quantises a block held by 4 consecutive lanes, 8 dimensions each (lane t of
 // the four: dimensions 8 t .. + 7).  Returns this lane's word; *scale gets the
 // bf16 bits.  Every lane of the warp calls it.
 __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t* scale) {
-    // the largest magnitude; its first holder's sign.  A NaN anywhere makes
-    // `bad` non-zero (x - x is 0 only for finite x).
-    float mx = x[0], bad = x[0] - x[0];
+    // the element of largest magnitude: the greater of the largest and the
+    // smallest, and of equal ones the first
+    float hi = x[0], lo = x[0];
+    uint64_t bad2 = 0;  // 0, or NaN of a NaN or an infinity
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        if (fabsf(x[i]) > fabsf(mx)) mx = x[i];
-        bad += x[i] - x[i];
+    for (int i = 0; i < 8; ++i) hi = fmaxf(hi, x[i]), lo = fminf(lo, x[i]);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) bad2 = f2_fma(pair(x[i], x[i + 1]), 0, bad2);
+    float bad, bad_hi;
+    unpair(bad2, bad, bad_hi);
+    bad += bad_hi;
+    float mx = hi > -lo ? hi : lo;
+    if (hi == -lo) {
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+            if (fabsf(x[i]) == hi) mx = x[i];
     }
-    bad = bad == 0.0f ? 0.0f : 1.0f;
+    const float inf = __uint_as_float(0x7f800000u);
+    if (bad != 0.0f) mx = inf;
     const int t = (int)(threadIdx.x & 3u);
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         const float other = __shfl_xor_sync(0xffffffffu, mx, o);
-        bad += __shfl_xor_sync(0xffffffffu, bad, o);
         const float a = fabsf(mx), b = fabsf(other);
         // equal magnitudes: the lower lane's (lower dimensions) sign
         if (b > a || (b == a && (t & o))) mx = other;
     }
-    const bool zero = fabsf(mx) < 7.8886090522101181e-31f;  // 2^-100
-    const __nv_bfloat16 db = __float2bfloat16_rn(zero ? 0.0f : __fdiv_rn(mx, -8.0f));
-    const float d = __bfloat162float(db);
-    const float inv = zero ? 0.0f : __frcp_rn(d);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float r = floorf(__fadd_rn(__fmul_rn(x[i], inv), 8.5f));
-        w |= (uint32_t)(int)fminf(fmaxf(r, 0.0f), 15.0f) << (4 * i);
+    if (fabsf(mx) == inf) {
+        *scale = 0x7fc0u;
+        return 0x88888888u;
     }
-    *scale = bad != 0.0f ? (uint16_t)0x7fc0u : reinterpret_cast<const uint16_t&>(db);
-    return bad != 0.0f ? 0x88888888u : w;
+    const bool zero = fabsf(mx) < 7.8886090522101181e-31f;  // 2^-100
+    const __nv_bfloat16 db = __float2bfloat16_rn(zero ? 0.0f : __fmul_rn(mx, -0.125f));
+    const float inv = zero ? 0.0f : __frcp_rn(__bfloat162float(db));
+    // |x (1/d)| is at most 8 (1 + 2^-8), so the sum lies in (0, 17): only 15 needs
+    // a clamp.  floor by adding 2^23 rounded down: the low bits are n, and the
+    // eight exponents that the shifts leave in the word add up to 0xfb000000
+    // (the products one by one: a packed product and a packed sum came out as one
+    // rounding, which moves values that lie on a boundary)
+    const uint64_t mid = pair(8.5f, 8.5f);
+    uint32_t w = 0u - 0xfb000000u;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float r0, r1;
+        unpair(f2_add(pair(__fmul_rn(x[i], inv), __fmul_rn(x[i + 1], inv)), mid), r0, r1);
+        w += __float_as_uint(__fadd_rd(fminf(r0, 15.5f), 8388608.0f)) << (4 * i);
+        w += __float_as_uint(__fadd_rd(fminf(r1, 15.5f), 8388608.0f)) << (4 * i + 4);
+    }
+    *scale = reinterpret_cast<const uint16_t&>(db);
+    return w;
 }
 
 // ------------------------------------------------- arithmetic on the blocks
@@ -157,19 +245,6 @@ __device__ __forceinline__ uint32_t nib_hi(uint32_t x) {
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(x));
     const __half2 h = __hadd2(reinterpret_cast<const __half2&>(r), __float2half2_rn(-1152.0f));
     return reinterpret_cast<const uint32_t&>(h);
-}
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
 // Nibbles I, I + 1 of x as (n - 8) 16^I, (n - 8) 16^(I + 1) in fp32: each is
 // masked in place and ORed into the mantissa of 2^23, and one packed addition
