@@ -44,13 +44,27 @@ def _np_ptr(a: np.ndarray):
 
 
 def _t_ptr(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+_current = None
+
+
+def _current_stream():
+    """Handle of the current device's current stream (torch.cuda.current_stream()
+    builds an object around it: 3 us of a call that takes 10)."""
+    global _current
+    if _current is None:
+        import torch
+        torch.cuda.init()
+        device, raw = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        _current = lambda: raw(device())  # noqa: E731
+    return _current()
 
 
 def _stream(stream):
     if stream is None:
-        import torch
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        return C.c_void_p(_current_stream())
     if isinstance(stream, int):
         return C.c_void_p(stream)
     return C.c_void_p(stream.cuda_stream)
@@ -348,11 +362,12 @@ def _bad(msg: str):
 
 def _heads(name: str, t, rows: int | None = None, hd: int | None = None):
     """Row and head stride of an activation tensor, checked."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
         _bad(f"{name} must be [rows, heads, head_dim] with a head's dimensions next to one another")
-    if rows is not None and t.shape[0] != rows or hd is not None and t.shape[2] != hd:
-        _bad(f"{name} is {tuple(t.shape)}: rows or head_dim differ from the other tensors'")
-    return t.stride(0), t.stride(1)
+    if rows is not None and shape[0] != rows or hd is not None and shape[2] != hd:
+        _bad(f"{name} is {tuple(shape)}: rows or head_dim differ from the other tensors'")
+    return stride
 
 
 def _i32(name: str, t, n: int | None = None):
@@ -367,15 +382,17 @@ def _rope_tables(cos_t, sin_t, rot_dim, head_dim):
     """(rot_dim, rows of the tables); without tables nothing is rotated."""
     if cos_t is None and sin_t is None and not rot_dim:
         return 0, 0
-    if cos_t is None or sin_t is None or cos_t.shape != sin_t.shape or cos_t.dim() != 2 or \
+    shape = () if cos_t is None else cos_t.shape
+    if sin_t is None or len(shape) != 2 or sin_t.shape != shape or \
             not (cos_t.is_contiguous() and sin_t.is_contiguous()) or str(cos_t.dtype) != "torch.float32" or \
-            str(sin_t.dtype) != "torch.float32":
+            sin_t.dtype != cos_t.dtype:
         _bad("cos and sin must be contiguous float32 tables [n_pos, rot_dim / 2]")
+    n_pos, half = shape
     if rot_dim is None:
-        rot_dim = 2 * cos_t.shape[1]
-    if 2 * cos_t.shape[1] != rot_dim or rot_dim > head_dim:
-        _bad(f"the tables hold {cos_t.shape[1]} angles per position: rot_dim {rot_dim}, head_dim {head_dim}")
-    return rot_dim, cos_t.shape[0]
+        rot_dim = 2 * half
+    if 2 * half != rot_dim or rot_dim > head_dim:
+        _bad(f"the tables hold {half} angles per position: rot_dim {rot_dim}, head_dim {head_dim}")
+    return rot_dim, n_pos
 
 
 def rope_table(rot_dim: int, n_pos: int, theta: float = 10000.0, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0,
