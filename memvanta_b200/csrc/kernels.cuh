@@ -242,7 +242,7 @@ struct AttnQ4Args {
     uint64_t out_stride;
     void* workspace = nullptr;  // attn_q4_workspace bytes; nullptr: stream-ordered scratch
 };
-// Scratch of one query row per sequence, for any context up to max_ctx.
+// Scratch that a call of these sizes takes (0: none).
 uint64_t attn_q4_workspace(int type, const AttnQ4Args& a);
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s);
 // attn_q4_prefill.cu : the same for chunks (q_start, one_seq), on tcgen05

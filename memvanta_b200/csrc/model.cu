@@ -1214,7 +1214,8 @@ void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, in
     if (kv_type == MV_KV_Q4_0) {
         mvb::AttnQ4Args a{};
         a.n_q = 1, a.n_head = m->nh, a.n_head_kv = m->nkv, a.hd = m->hd, a.page = m->page, a.max_ctx = m->n_ctx;
-        m->q4_workspace = dalloc<uint8_t>(m, mvb::attn_q4_workspace(MV_TYPE_F32, a));
+        const uint64_t bytes = mvb::attn_q4_workspace(MV_TYPE_F32, a);
+        if (bytes) m->q4_workspace = dalloc<uint8_t>(m, bytes);
     }
     {
         const char* env = std::getenv("MV_ATTN_SPLIT");

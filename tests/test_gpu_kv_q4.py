@@ -375,6 +375,33 @@ def test_decode_long(cuda, n_seq, heads, H, hd, ctx):
     assert torch.equal(got, mv.paged_attn_q4(*args))
 
 
+@pytest.mark.parametrize("n_seq,heads,H,hd,longest,dtype", [
+    (1, 2, 1, 128, 1, "float32"), (2, 8, 4, 128, 130, "float16"), (5, 24, 8, 128, 1200, "bfloat16"),
+    (27, 9, 3, 64, 700, "float32"), (55, 4, 4, 256, 90, "float16"), (110, 4, 1, 128, 300, "float32"),
+    (100, 4, 4, 128, 60, "bfloat16"), (150, 3, 3, 64, 260, "float32"), (1, 20, 1, 256, 4000, "bfloat16")])
+def test_decode_few_and_many_units(cuda, n_seq, heads, H, hd, longest, dtype):
+    """From one (sequence, kv head) to more than the GPU holds at once: contexts
+    of no token (and fewer), of one, and up to the longest in between."""
+    import torch
+    rng = np.random.default_rng(n_seq)
+    ctx = rng.integers(1, longest + 1, n_seq).astype(np.int32)
+    ctx[0] = longest
+    if n_seq > 1:
+        ctx[n_seq // 2], ctx[-1] = 0, 1
+    if n_seq > 4:
+        ctx[3] = -5
+    page = 13
+    t, total = scattered(np.maximum(ctx, 0), page, 80)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 81)
+    q = randn((n_seq, heads, hd), 82, dtype, 1.5)
+    args = (q, kp, vp, ks, vs, torch.from_numpy(t).cuda(), torch.from_numpy(ctx).cuda(), longest)
+    got = mv.paged_attn_q4(*args)
+    want, bound = attention64(q, kp, ks, vp, vs, t, range(n_seq), ctx, page, hd ** -0.5)
+    check_attention(got, want, bound)
+    assert not got[torch.from_numpy(ctx <= 0).cuda()].any()
+    assert torch.equal(got, mv.paged_attn_q4(*args))
+
+
 def test_decode_garbage_past_the_context(cuda):
     """NaN scales, wild pages and stale nibbles past ctx_len change nothing; a
     page that does not exist is left out; max_ctx cuts."""
