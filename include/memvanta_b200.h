@@ -87,9 +87,9 @@ MV_API int mv_version(void);
 MV_API int mv_binary_arch(int* out);
 /* Synchronises `stream` and reports MV_ERR_TIMEOUT if a kernel with bounded
  * device-side waits (the tensor-core GEMMs of mv_gemm with MV_ACT_Q8 and of
- * the model's prefill, the decode GEMV's and the cluster attention's
- * exchanges between CTAs) gave up a wait since the last check -- its outputs
- * are then invalid.  Host-pointer calls and the model's prefill check this
+ * the model's prefill, mv_paged_attn_q4_prefill, the decode GEMV's and the
+ * cluster attention's exchanges between CTAs) gave up a wait since the last
+ * check -- its outputs are then invalid.  Host-pointer calls and the model's prefill check this
  * themselves.  No counterpart in the reference. */
 MV_API int mv_stream_status(void* stream);
 /* Test hook for the bounded waits (no counterpart in the reference): the

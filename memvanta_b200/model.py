@@ -4,7 +4,8 @@ Mirrors the reference's public class (include/memvanta/llama_model.hpp:100-113):
 ``LlamaModel(path, threads, ctx, page_tokens, kv_type)``, ``forward``,
 ``prefill``, ``generate``, ``reset``, ``position``, ``kv_bytes_allocated``.
 ``threads`` is accepted for signature compatibility and ignored (the GPU
-parallelises internally).
+parallelises internally).  ``kv_type`` is any ``KV_*``; ``KV_Q4_0`` (4 bits a
+value, one GPU) has no counterpart in the reference and is not held to its order.
 """
 from __future__ import annotations
 
