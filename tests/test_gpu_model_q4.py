@@ -5,6 +5,7 @@ three routes: a prompt, one token at a time, a batch of sequences.
 from __future__ import annotations
 
 import ctypes as C
+import dataclasses
 import os
 import tempfile
 
@@ -142,6 +143,53 @@ def test_model_follows_the_64_bit_model(cuda, tmp):
         assert np.max(np.abs(again - first)) <= TOL64 * np.max(np.abs(first))
     finally:
         m.close()
+
+
+@pytest.mark.gpu
+def test_long_prompt_in_chunks(cuda, tmp):
+    """A prompt of several merged chunks, which overlap on two streams."""
+    shape = dataclasses.replace(FULL, n_ctx=1400)
+    path = written(tmp, "long.gguf", shape, 33)
+    prompt = np.random.default_rng(8).integers(0, shape.vocab, size=1300).astype(np.int32)
+    ref = Model64(path, shape)
+    m = mv.LlamaModel(path, ctx_override=1400, kv_page_tokens=64, kv_type=mv.KV_Q4_0)
+    try:
+        got = m.prefill(prompt, 128).copy()
+        want = [ref.forward(int(t)) for t in prompt][-1]
+        assert np.max(np.abs(got - want)) <= TOL64 * np.max(np.abs(want))
+        for _ in range(3):
+            tok = int(np.argmax(want))
+            got, want = m.forward(tok).copy(), ref.forward(tok)
+            assert np.max(np.abs(got - want)) <= TOL64 * np.max(np.abs(want))
+    finally:
+        m.close()
+
+
+@pytest.mark.gpu
+def test_many_sequences(cuda, tmp):
+    """A set of 70 sequences against the 64-bit model, a few of them at a time."""
+    path = written(tmp, "full.gguf", FULL, 31)
+    rng = np.random.default_rng(9)
+    prompts = [rng.integers(0, FULL.vocab, size=1 + 3 * i % 50).astype(np.int32) for i in range(70)]
+    steps = rng.integers(0, FULL.vocab, size=(4, 70)).astype(np.int32)
+    m = mv.LlamaModel(path, ctx_override=128, kv_page_tokens=16, kv_type=mv.KV_Q4_0)
+    try:
+        S = m.open_sequences(70, 64)
+        try:
+            for i, p in enumerate(prompts):
+                S.prefill(i, p, 32)
+            got = [S.forward(t).copy() for t in steps]
+        finally:
+            S.close()
+    finally:
+        m.close()
+    for i in (0, 1, 17, 40, 69):
+        ref = Model64(path, FULL)
+        for t in prompts[i]:
+            ref.forward(int(t))
+        for k in range(4):
+            want = ref.forward(int(steps[k, i]))
+            assert np.max(np.abs(got[k][i] - want)) <= TOL64 * np.max(np.abs(want)), (i, k)
 
 
 @pytest.mark.gpu
