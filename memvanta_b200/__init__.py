@@ -47,7 +47,16 @@ def _t_ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_current = None
+_torch_module = _current = None
+
+
+def _torch():
+    """torch, imported with the first call that takes its tensors."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _current_stream():
@@ -64,7 +73,7 @@ def _current_stream():
 
 def _stream(stream):
     if stream is None:
-        return C.c_void_p(_current_stream())
+        return _current_stream()
     if isinstance(stream, int):
         return C.c_void_p(stream)
     return C.c_void_p(stream.cuda_stream)
@@ -373,7 +382,7 @@ def _heads(name: str, t, rows: int | None = None, hd: int | None = None):
 def _i32(name: str, t, n: int | None = None):
     if t is None:
         return None
-    if str(t.dtype) != "torch.int32" or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.dtype is not _torch().int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
         _bad(f"{name} must be a contiguous int32 tensor" + ("" if n is None else f" of {n} elements"))
     return t.data_ptr()
 
@@ -384,8 +393,8 @@ def _rope_tables(cos_t, sin_t, rot_dim, head_dim):
         return 0, 0
     shape = () if cos_t is None else cos_t.shape
     if sin_t is None or len(shape) != 2 or sin_t.shape != shape or \
-            not (cos_t.is_contiguous() and sin_t.is_contiguous()) or str(cos_t.dtype) != "torch.float32" or \
-            sin_t.dtype != cos_t.dtype:
+            not (cos_t.is_contiguous() and sin_t.is_contiguous()) or cos_t.dtype is not _torch().float32 or \
+            sin_t.dtype is not cos_t.dtype:
         _bad("cos and sin must be contiguous float32 tables [n_pos, rot_dim / 2]")
     n_pos, half = shape
     if rot_dim is None:
@@ -462,7 +471,7 @@ def _pool_pages(kv_type: int, pages, scales, page: int, n_head_kv: int, head_dim
     if not pages.is_contiguous() or (scales is not None and not scales.is_contiguous()):
         _bad("cache pages and scales must be contiguous")
     per = page * kv_dim // 2 if kv_type == KV_Q4_0 else page * kv_dim * _KV_ELEMENT[kv_type]
-    n = pages.numel() * pages.element_size() // per if per else 0
+    n = pages.nbytes // per if per else 0
     if kv_type >= KV_Q8 and scales is not None:
         need = n * page * (1 if kv_type == KV_Q8 else kv_dim // 32)
         if scales.numel() < need or scales.element_size() != (2 if kv_type == KV_Q4_0 else 4):

@@ -120,6 +120,8 @@ _lib = None
 def load(path: str = LIB_PATH) -> C.CDLL:
     """Load (once) and return the library with every signature declared."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(path):

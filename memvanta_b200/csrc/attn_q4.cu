@@ -4,6 +4,16 @@
 // over the first ctx_len[r] cached tokens of the row's sequence, in one pass
 // with the running maximum m and sum.  A row with no tokens gives zeros; what
 // lies past ctx_len, or on a page that does not exist, is never used.
+//
+// Measured (back-to-back launches; 2 x (hd / 2 + hd / 16) bytes a token and kv head):
+//   1 x 768 tokens, 32 kv heads x 128, fp32 queries          6.1 us  (latency)
+//   1 x 131,071 tokens, 8 kv heads x 128, 32 heads fp32      55.9 us  151 MB: 2.7 TB/s, 0.41 of HBM's
+//   64 x 64..768 tokens, 32 heads x 128 fp32                 45.5 us  2.1 TB/s
+//   48 x 1..16,384 tokens, 8 kv heads x 64, 64 heads fp16    66.4 us  2.3 TB/s
+// Long contexts are bound by instructions -- 436 for 16 tokens of head_dim 128, half
+// of the integer pipe's time, a third of the tensor cores' -- and not by memory:
+// the same ring without its arithmetic takes 24.5 us for the 55.9.
+// Tried: two stages to a ring, 80 to 96 registers, more and smaller CTAs (slower).
 #include <cuda_runtime.h>
 
 #include <algorithm>

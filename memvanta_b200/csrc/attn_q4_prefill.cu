@@ -28,6 +28,25 @@
 // value blocks enter as zeros, and the rows that see one get NaN in its
 // dimensions at the end.
 // Every wait is bounded (tc.cuh).
+//
+// Tiles: a query tile is as high as the MMA (128 lanes of TMEM).  64 tokens (32 for
+// head_dim 256) are what two buffers of scores, the outputs and, for fp32, the
+// weights' second parts leave room for in TMEM; two query tiles share an expanded
+// tile where that fits (half precision, head_dim up to 128) and still gives every
+// SM a CTA.  The last query tiles start first: they see the most tokens.
+// Measured (back-to-back launches):
+//   512 rows, 32 heads x 128, fp32                          24.4 us
+//   2,048 rows after 14,336, 32 heads / 8 x 128, bf16        690 us  515 GFLOP: 0.75 PFLOP/s, 0.45 of bf16
+//   7 x 331 rows after 1,500, 16 heads / 4 x 256, fp16       88 us  0.21 PFLOP/s
+// Bound by latency: per token tile 1.57 us (fp32), 1.12 us (half precision, head_dim
+// 128; two query tiles 2.7 us), 2.5 us (head_dim 256, 32 tokens twice), of which the
+// MMAs take 0.5 to 0.6 us a query tile; the rest is the chain scores - maximum -
+// weights - outputs of 64 exponentials a thread and the hand-offs.  9 us (fp32) or
+// 6 us (half) are launch, queries, first tile and outputs; and the last wave of
+// CTAs is part empty (256 CTAs and 308 on 148 SMs).
+// Tried: one warp issuing all MMAs in order (870 us for the 690), one lane polling
+// for its warp (+8%), a single buffer of scores (fp32 +13%), outputs through shared
+// memory in whole lines (1 us less at the end, 4% more in the loop: registers).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -79,8 +98,8 @@ struct Pf {
     static constexpr int kOffMisc = kOffBar + kBars * 8;
     // exponents of the query rows [NQ][128]; factor 2^-e [kRing], token masks
     // [kRing][2], blocks that are not finite: any [kRing][2], which tokens
-    // [kRing][2][NB]; TMEM base, abort flag, tokens
-    static constexpr int kSmem = kOffMisc + NQ * kRows * 4 + kRing * (4 + 8 + 8 + 8 * NB) + 12 + 1024;
+    // [kRing][2][NB]; TMEM base, abort flag, most tokens of a softmax warp's rows
+    static constexpr int kSmem = kOffMisc + NQ * kRows * 4 + kRing * (4 + 8 + 8 + 8 * NB) + 8 + NQ * 16 + 1024;
     static constexpr int kExpand = NQ == 2 ? 4 : 8;  // warps
     static constexpr int kThreads = NQ * 128 + kExpand * 32 + 2 * NQ * 32;
     // TMEM columns of a query tile: two buffers of NT scores, taken by the
@@ -206,61 +225,13 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         tc::mbar_init(t_free, 128);  // a tile's first OT columns are taken out
         tc::mbar_fence_init();
         *abort_flag = 0;
-        *most = 0;
     }
     constexpr int kMmaWarp = NQ * 4 + C::kExpand;
     if (warp == kMmaWarp) {
         tc::tmem_alloc(tc::smem_u32(tmem_at), C::kTmem);
         tc::tmem_relinquish();
     }
-    __syncthreads();
-
-    // ---- queries into shared memory, 8 lanes to a row: row m of tile q is query
-    // row m / nh, head m % nh
-    if (warp < kMmaWarp) {
-        constexpr int kPer = HD / 64;  // 8-dimension units of a lane
-#pragma unroll 1
-        for (int r = warp * 4 + lane / 8; r < NQ * kRows; r += kMmaWarp * 4) {
-            const int tile = r / kRows, m = r % kRows, u0 = lane % 8;
-            const int64_t row = row0 + tile * p.rpt + m / nh;
-            const bool there_is = m / nh < p.rpt && row < seq1;
-            const T* src = static_cast<const T*>(a.q) + (there_is ? row * (int64_t)a.q_stride + (int64_t)(h0 + m % nh) * HD : 0);
-            float x[kPer][8], mx = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                load_n<8, true>(src + 8 * (u0 + 8 * k), x[k]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (!there_is) x[k][i] = 0.0f;
-                    mx = fmaxf(mx, fabsf(x[k][i]));
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            // times 2^e: the largest below 2^15
-            const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
-            const float up = pow2i(e);
-            if (u0 == 0) q_exp[r] = e;
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                float lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[k][i] *= up;
-                    lo[i] = x[k][i] - __half2float(__float2half_rn(x[k][i]));
-                }
-                // dims of a unit in the order of the expanded keys: 0 4 1 5 2 6 3 7
-                uint8_t* at = sm + tile * C::kParts * C::kQ + k * kRows * 128 + sw128(m, u0);
-                *reinterpret_cast<uint4*>(at) = make_uint4(pack_half2(x[k][0], x[k][4]), pack_half2(x[k][1], x[k][5]),
-                                                           pack_half2(x[k][2], x[k][6]), pack_half2(x[k][3], x[k][7]));
-                if constexpr (kTwo)
-                    *reinterpret_cast<uint4*>(at + C::kQ) = make_uint4(pack_half2(lo[0], lo[4]), pack_half2(lo[1], lo[5]),
-                                                                       pack_half2(lo[2], lo[6]), pack_half2(lo[3], lo[7]));
-            }
-        }
-        tc::fence_proxy_async_smem();
-    }
-    // softmax thread m of tile q holds that row
+    // softmax thread m of tile q holds row m of it, query m / nh, head m % nh
     const int q_of = warp / 4, m_of = (warp % 4) * 32 + lane;
     int ctx = 0, my_head = 0;
     int64_t my_row = -1;
@@ -272,13 +243,16 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             ctx = max(0, min(a.ctx_len[r], (int)a.max_ctx));
         }
         const int top = __reduce_max_sync(0xffffffffu, ctx);
-        if (lane == 0 && top) atomicMax(most, top);
+        if (lane == 0) most[warp] = top;
     }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_at;
-    const int tokens = *most, tiles = (tokens + NT - 1) / NT;
+    int tokens = 0;
+#pragma unroll
+    for (int w = 0; w < NQ * 4; ++w) tokens = max(tokens, most[w]);
+    const int tiles = (tokens + NT - 1) / NT;
 
     if (warp >= kMmaWarp) {
         // ----------------------------------------------------- MMA issuers
@@ -296,6 +270,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                 // scores, into the buffer whose weights, of two tiles before, have been multiplied
                 constexpr uint32_t id = idesc(0, kRows, NT);
                 const uint32_t qb = sb + q * C::kParts * C::kQ;
+                asm volatile("bar.sync %0, 160;" ::"r"(1 + q) : "memory");  // the tile's queries are there
                 for (int i = 0; i < tiles; ++i) {
                     if (!wait(k_full(i & 1), i >> 1, 40)) break;
                     if (i >= 2 && !wait(o_done(q, i), (i - 2) >> 1, 41)) break;
@@ -304,7 +279,8 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                     for (int part = 0; part < C::kParts; ++part)
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k)
-                            mma_f16_ss(d, tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
+                            mma_f16_ss(d,
+                                       tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
                                        tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id, part || k);
                     commit(s_full(q, i));
                     if (lane == 0) tc::mbar_arrive(s_full(q, i));
@@ -494,13 +470,74 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         }
     } else {
         // ------------------------------------------------------- softmax
+        // First this warp's 32 query rows, 8 lanes to a row, into shared memory (the
+        // cache's first tile is fetched and expanded meanwhile)
+        constexpr int kPer = HD / 64;                                        // 8-dimension units of a lane
+        constexpr int kRows4 = std::min(8, (sizeof(T) == 4 ? 8 : 16) / kPer);  // times 4 rows in flight
+        const int u0 = lane % 8;
+#pragma unroll 1
+        for (int it = 0; it < 8; it += kRows4) {
+            Held<T, 8, true> in[kRows4][kPer];
+            bool there_is[kRows4];
+#pragma unroll
+            for (int k = 0; k < kRows4; ++k) {
+                const int m = (warp % 4) * 32 + (it + k) * 4 + lane / 8;
+                const int64_t row = row0 + q_of * p.rpt + m / nh;
+                there_is[k] = m / nh < p.rpt && row < seq1;
+                const int64_t at = there_is[k] ? row * (int64_t)a.q_stride + (int64_t)(h0 + m % nh) * HD : 0;
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) in[k][u].load(static_cast<const T*>(a.q) + at + 8 * (u0 + 8 * u));
+            }
+#pragma unroll
+            for (int k = 0; k < kRows4; ++k) {
+                const int m = (warp % 4) * 32 + (it + k) * 4 + lane / 8;
+                float x[kPer][8], mx = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) {
+                    in[k][u].get(x[u]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (!there_is[k]) x[u][i] = 0.0f;
+                        mx = fmaxf(mx, fabsf(x[u][i]));
+                    }
+                }
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                // times 2^e: the largest below 2^15
+                const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+                const float up = pow2i(e);
+                if (u0 == 0) q_exp[q_of * kRows + m] = e;
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) {
+                    float lo[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[u][i] *= up;
+                        lo[i] = x[u][i] - __half2float(__float2half_rn(x[u][i]));
+                    }
+                    // dims of a unit in the order of the expanded keys: 0 4 1 5 2 6 3 7
+                    uint8_t* to = sm + q_of * C::kParts * C::kQ + u * kRows * 128 + sw128(m, u0);
+                    *reinterpret_cast<uint4*>(to) =
+                        make_uint4(pack_half2(x[u][0], x[u][4]), pack_half2(x[u][1], x[u][5]),
+                                   pack_half2(x[u][2], x[u][6]), pack_half2(x[u][3], x[u][7]));
+                    if constexpr (kTwo)
+                        *reinterpret_cast<uint4*>(to + C::kQ) =
+                            make_uint4(pack_half2(lo[0], lo[4]), pack_half2(lo[1], lo[5]), pack_half2(lo[2], lo[6]),
+                                       pack_half2(lo[3], lo[7]));
+                }
+            }
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();  // the exponents, too
+        if (tiles) asm volatile("bar.arrive %0, 160;" ::"r"(1 + q_of) : "memory");
         const uint32_t tm = tmem + q_of * C::kCols + ((uint32_t)(warp % 4) << 21);  // this warp's 32 lanes
         const float c_row = fmaxf(a.scale * 1.44269504088896341f * pow2i(-q_exp[q_of * kRows + m_of]), 1e-37f);
         float m_run = -INFINITY, l = 0.0f;
         uint32_t bad = 0;  // blocks of dimensions in which this row sees values that are not finite
         bool ok = true;
         auto wait = [&](uint32_t bar, int parity, int site) {
-            const bool got = __all_sync(0xffffffffu, tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site));
+            const bool got = __all_sync(0xffffffffu,
+                                        tc::mbar_wait(bar, (uint32_t)parity & 1u, abort_flag, &g_q4_status, site));
             if (got) tc::tc_fence_after();
             return got;
         };
