@@ -475,6 +475,15 @@ def other_configs():
     return out
 
 
+NO_REFERENCE = "the reference's own bench is not built here (its sources are not present)"
+
+
+def reference_bench() -> bool:
+    sys.path.insert(0, os.path.join(ROOT, "oracle"))
+    from oracle import REF_REAL_BENCH
+    return os.path.exists(REF_REAL_BENCH)
+
+
 def run_llama7b_cpu(threads=None, prompt=512, gen=16):
     """The reference's own memvanta_real_bench (oracle/_ref, built from the
     unmodified sources) on this host's cores: pp<prompt> and tg<gen> tok/s."""
@@ -786,6 +795,9 @@ def main_llama7b(args, world, rank, local):
             return
         # the same workload as our arm: pp512 in batches of 32, then K = --steps
         # greedy decode tokens after the reference bench's 128-token seed prefill
+        if not reference_bench():
+            print(json.dumps({"impl": "reference", "unavailable": NO_REFERENCE}), flush=True)
+            return
         cpu = run_llama7b_cpu(prompt=L7_PP, gen=args.steps)
         line = {"impl": "reference", "metric": metric, "value": cpu["tg"], "unit": unit, "n_gpus": args.gpus,
                 "steps": args.steps, "warmup": args.warmup, "higher_is_better": True, "dtype": "q4_0/q8",
@@ -810,7 +822,9 @@ def main_llama7b(args, world, rank, local):
     extra = other_configs() if world == 1 else {}
     peaks = measured_peaks()
     cpu = None
-    if world == 1:
+    if world == 1 and not reference_bench():
+        cpu = {"unavailable": NO_REFERENCE}
+    elif world == 1:
         c = run_llama7b_cpu()
         cpu = {"value": c["tg"], "unit": unit, "cores": c["threads"], "kind": "reference", "sample": c["sample"],
                "pp_tok_s": c["pp"]}
