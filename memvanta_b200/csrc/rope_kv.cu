@@ -14,12 +14,13 @@
 //   append to F16, 2,048 rows, 32 + 2 x 8 heads x 128 fp16       9.3 us  5.4 TB/s
 //   append to Q4_0, 4,093 rows, 32 + 2 x 32 heads x 128 fp32    67.9 us  4.2 TB/s
 //   rotation or append of 64 rows                          2.0 and 3.3 us
+//   reading 4,093 rows x 32 x 128 of Q4_0 back as fp16         10.9 us  4.0 TB/s
 // The Q4_0 append is bound by instructions: 500 for 16 dimensions of K and V, half
 // of them the block's scale and the rounding of its nibbles (63% of the issue
 // slots are taken, 36% of the memory's time).  Small calls are a launch and three
 // loads that wait on one another (position, page, angle).
 // Tried: a thread for several heads, so that the row's part is done once
-// (113 to 127 us with its reads, 101 as it is: fewer threads hide less), lines
+// (113 to 127 us with its reads, 101 without: fewer threads hide less), lines
 // asked for into L2 a wave ahead (no change), 8-byte accesses for half types
 // (29 us for the 27.7).
 #include <cuda_runtime.h>
@@ -442,37 +443,54 @@ __global__ void __launch_bounds__(kThreads) rope_kv_append_q8_kernel(RopeAppendA
 }
 
 // ----------------------------------------------------------------- read
-// Rows of one pool as out[row][kv head][hd]; a skipped row reads zeros.
-template <class T, int KVT>
+// Rows of one pool as out[row][kv head][hd]; a skipped row reads zeros.  A thread
+// takes 8 dimensions, of Q4_0 B times that: the same quarter of B blocks that
+// follow one another, whose words and scales do too (4,093 rows x 32 x 128 to fp16:
+// 10.9 us with B = 2, 15.2 us with 1).
+template <class T, int KVT, int B>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, Items t, Div page, int64_t n_rows) {
     int64_t r;
     int h, j;
     if (!place(t, blockIdx.x, n_rows, &r, &h, &j)) return;
-    const int hd = (int)a.hd, H = (int)a.n_head_kv, d = j * 8;
+    const int hd = (int)a.hd, H = (int)a.n_head_kv, d = B == 1 ? j * 8 : j / 4 * (32 * B) + j % 4 * 8;
     int slot = 0;
     const int64_t pg = kv_slot_page(a.rows, page, r, &slot);
-    float y[8];
+    float y[B][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = 0.0f;
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[b][k] = 0.0f;
     if (pg >= 0) {
         const Spot s = spot_of<KVT>(pg, slot, (int)a.rows.page, H, h, hd, d);
         if constexpr (KVT == 0) {
-            load_n<8, true>(static_cast<const float*>(a.pages) + s.at, y);
+            load_n<8, true>(static_cast<const float*>(a.pages) + s.at, y[0]);
         } else if constexpr (KVT == 1) {
-            load_n<8, true>(static_cast<const __half*>(a.pages) + s.at, y);
+            load_n<8, true>(static_cast<const __half*>(a.pages) + s.at, y[0]);
         } else if constexpr (KVT == kKvQ4) {
-            const uint32_t w = static_cast<const uint32_t*>(a.pages)[s.at];
-            const float sc = bf16_bits_to_f32(static_cast<const uint16_t*>(a.scales)[s.scale]);
+            uint32_t w[B];
+            float sc[B];
+            if constexpr (B == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint32_t*>(a.pages) + s.at);
+                const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.scales) + s.scale);
+                w[0] = v.x, w[1] = v.y;
+                sc[0] = __uint_as_float(u << 16), sc[1] = __uint_as_float(u & 0xffff0000u);
+            } else {
+                w[0] = static_cast<const uint32_t*>(a.pages)[s.at];
+                sc[0] = bf16_bits_to_f32(static_cast<const uint16_t*>(a.scales)[s.scale]);
+            }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = (float)((int)(w >> (4 * k) & 15u) - 8) * sc;
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[b][k] = (float)((int)(w[b] >> (4 * k) & 15u) - 8) * sc[b];
         } else {
             const float sc = static_cast<const float*>(a.scales)[KVT == 2 ? pg * (int64_t)a.rows.page + slot : s.scale];
             const int8_t* q = static_cast<const int8_t*>(a.pages) + s.at;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = (float)q[k] * sc;
+            for (int k = 0; k < 8; ++k) y[0][k] = (float)q[k] * sc;
         }
     }
-    store_n<8, true>(static_cast<T*>(a.out) + (r * H + h) * hd + d, y);
+#pragma unroll
+    for (int b = 0; b < B; ++b) store_n<8, true>(static_cast<T*>(a.out) + (r * H + h) * hd + d + 32 * b, y[b]);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -508,7 +526,8 @@ cudaError_t append_kv(const RopeAppendArgs& a, cudaStream_t s) {
 }
 template <class T>
 cudaError_t read_kv(const KvReadArgs& a, uint64_t rows, cudaStream_t s) {
-    const Items t = items_of(rows, a.n_head_kv, a.hd / 8);
+    const bool two = a.kv_type == kKvQ4 && a.hd % 64 == 0;
+    const Items t = items_of(rows, a.n_head_kv, a.hd / (two ? 16 : 8));
     const Div page = div_by(a.rows.page);
     if (t.blocks > kMaxGrid) return cudaErrorInvalidConfiguration;
     auto go = [&](auto kernel) {
@@ -516,11 +535,11 @@ cudaError_t read_kv(const KvReadArgs& a, uint64_t rows, cudaStream_t s) {
         return cudaGetLastError();
     };
     switch (a.kv_type) {
-        case 0: return go(kv_read_kernel<T, 0>);
-        case 1: return go(kv_read_kernel<T, 1>);
-        case 2: return go(kv_read_kernel<T, 2>);
-        case 3: return go(kv_read_kernel<T, 3>);
-        default: return go(kv_read_kernel<T, kKvQ4>);
+        case 0: return go(kv_read_kernel<T, 0, 1>);
+        case 1: return go(kv_read_kernel<T, 1, 1>);
+        case 2: return go(kv_read_kernel<T, 2, 1>);
+        case 3: return go(kv_read_kernel<T, 3, 1>);
+        default: return two ? go(kv_read_kernel<T, kKvQ4, 2>) : go(kv_read_kernel<T, kKvQ4, 1>);
     }
 }
 
