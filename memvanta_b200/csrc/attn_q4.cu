@@ -6,13 +6,13 @@
 // lies past ctx_len, or on a page that does not exist, is never used.
 //
 // Measured (back-to-back launches; 2 x (hd / 2 + hd / 16) bytes a token and kv head):
-//   1 x 768 tokens, 32 kv heads x 128, fp32 queries          6.1 us  (latency)
-//   1 x 131,071 tokens, 8 kv heads x 128, 32 heads fp32      55.9 us  151 MB: 2.7 TB/s, 0.41 of HBM's
-//   64 x 64..768 tokens, 32 heads x 128 fp32                 45.5 us  2.1 TB/s
+//   1 x 768 tokens, 32 kv heads x 128, fp32 queries          6.6 us  (latency)
+//   1 x 131,071 tokens, 8 kv heads x 128, 32 heads fp32      59.5 us  151 MB: 2.5 TB/s, 0.39 of HBM's
+//   64 x 64..768 tokens, 32 heads x 128 fp32                 48.3 us  1.9 TB/s
 //   48 x 1..16,384 tokens, 8 kv heads x 64, 64 heads fp16    66.4 us  2.3 TB/s
-// Long contexts are bound by instructions -- 436 for 16 tokens of head_dim 128, half
+// Long contexts are bound by instructions -- some 440 for 16 tokens of head_dim 128, half
 // of the integer pipe's time, a third of the tensor cores' -- and not by memory:
-// the same ring without its arithmetic takes 24.5 us for the 55.9.
+// the same ring without its arithmetic takes 24.5 us for the 59.5.
 // Tried: two stages to a ring, 80 to 96 registers, more and smaller CTAs (slower).
 #include <cuda_runtime.h>
 
@@ -113,6 +113,8 @@ struct Q4Tile {
     static constexpr int kScale = TT * NB * 2;
     static constexpr int kBytes = 2 * 2048 + 2 * kScale;  // K, V, K scales, V scales
     static constexpr int kRing = kStages * kBytes;
+    static constexpr int kTotal = HD * 8 * 4;  // a warp's outputs so far: 16 x 8 per 16 dimensions, both parts
+    static constexpr int kFlush = 32 / NJ;     // stages between their sums
     // unit u of token row r sits at u ^ swz(r): the fragment loads are then
     // free of bank conflicts (8 rows x 16 bytes, or 4 rows 2 apart)
     static __device__ __forceinline__ int swz(int r) { return (r >> (U == 8 ? 0 : U == 4 ? 1 : 2)) & (U - 1); }
@@ -397,6 +399,13 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     const uint64_t bias0 = held_pair(-8388616.0f, -8388736.0f), bias1 = held_pair(-8390656.0f, -8421376.0f);
     const uint32_t first = g >= 4 ? 0xffffe000u : 0u;
     float o[NB][2][4];  // [block][dims 4g + 2 mu + {0, 1}][heads 2t, 2t + 1 of rows g, g + 8]
+    // The tensor core cuts its running sums instead of rounding them (2e-8 to 4e-8 of
+    // the sum an MMA).  fp32 queries: every 32 MMAs, and whenever the reference
+    // moves, the outputs are added, rounded, to totals in shared memory and start
+    // from zero.  131,071 tokens: relative error 1.6e-6 to 2.3e-6 without, 4.5e-7 to
+    // 8.8e-7 so (every 16: 3.6e-7 to 5.0e-7), for 59.5 us instead of 56.0.
+    float4* total = reinterpret_cast<float4*>(smem + kWarps * X::kRing + warp * X::kTotal) + lane;
+    bool held = false;  // something is in the totals
     float m_run = -INFINITY, l_run = 0.0f;
     uint32_t off = 0, refill = (kStages - 1) * X::kBytes;  // of the stage computed, and of the one copied into
     if (CL && !count && lane < sp.heads)  // nothing of this warp's counts
@@ -450,6 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
                 for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
         m_run = -INFINITY;
         l_run = 0.0f;
+        held = false;
         for (; at.stage < end; ++at.stage, ++n) {
             cp_async_wait<kStages - 2>();
             __syncwarp();
@@ -510,7 +520,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
             // The reference m follows the maximum only once that is 2^8 above it:
             // weights up to 2^8 do no harm, and the outputs are seldom rescaled.
             mx *= c_h;
-            if (__any_sync(0xffffffffu, mx > m_run + 8.0f)) {
+            const bool sum = kTwo && at.stage != from && (at.stage - from) % X::kFlush == 0;
+            if (sum || __any_sync(0xffffffffu, mx > m_run + 8.0f)) {
                 const float m_new = fmaxf(m_run, mx), alpha = m_new == -INFINITY ? 0.0f : ex2(m_run - m_new);
                 l_run *= alpha;
                 const uint64_t aa =
@@ -518,10 +529,24 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2)
-                            unpair(tc::f2_mul(pair(o[b][m][i], o[b][m][i + 1]), aa), o[b][m][i], o[b][m][i + 1]);
+                    for (int m = 0; m < 2; ++m) {
+                        float(&x)[4] = o[b][m];
+                        if (kTwo && at.stage == from) continue;  // zeros
+                        uint64_t u = pair(x[0], x[1]), v = pair(x[2], x[3]);
+                        if constexpr (kTwo) {
+                            if (held) {
+                                const float4 y = total[(2 * b + m) * 32];
+                                u = f2_add(u, pair(y.x, y.y)), v = f2_add(v, pair(y.z, y.w));
+                            }
+                        }
+                        unpair(tc::f2_mul(u, aa), x[0], x[1]);
+                        unpair(tc::f2_mul(v, aa), x[2], x[3]);
+                        if constexpr (kTwo) {
+                            total[(2 * b + m) * 32] = make_float4(x[0], x[1], x[2], x[3]);
+                            x[0] = x[1] = x[2] = x[3] = 0.0f;
+                        }
+                    }
+                held = at.stage != from;
                 m_run = m_new;
             }
             const float m_use = m_run == -INFINITY ? 0.0f : m_run;
@@ -586,6 +611,16 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         }
 
         // ---- the unit's end, or the run's
+        if constexpr (kTwo) {
+            if (held)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const float4 y = total[(2 * b + m) * 32];
+                        o[b][m][0] += y.x, o[b][m][1] += y.y, o[b][m][2] += y.z, o[b][m][3] += y.w;
+                    }
+        }
         const bool done = at.stage == at.stages;
         const bool whole = !CL && done && from == 0;
         float l = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
@@ -783,7 +818,7 @@ template <class T, int HD, bool PACK>
 cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     using X = Q4Tile<HD>;
     constexpr int kHeads = PACK ? 4 : 8;
-    const int smem = kWarps * X::kRing + kWarps * kStages * 8;
+    const int smem = kWarps * (X::kRing + (sizeof(T) == 4 ? X::kTotal : 0));
     auto kernel = attn_q4_decode_kernel<T, HD, PACK, false>;
     ensure_smem_attr(kernel, smem);
     static const uint64_t slots = resident_ctas(reinterpret_cast<const void*>(kernel), kWarps * 32, smem);
@@ -802,7 +837,8 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     // Short contexts of few units: a cluster a unit, of 8 CTAs or the fewest that give
     // a warp one stage, while the GPU holds them all at once and none has more than
     // kShort stages to a warp.  Runs over all units and a second kernel that joins
-    // them, against this (fp32 queries, head_dim 128):
+    // them, against this (fp32 queries, head_dim 128; both 3 to 6% less than with the
+    // rounded totals above):
     //    768 tokens, 32 units     9.3 ->  6.1 us     4,096 tokens, 32 units  16.2 -> 11.1 us
     //    1,000 tokens, 64 units  15.1 ->  8.4 us     4,000 tokens, 64 units  23.6 -> 17.8 us
     //    250 tokens, 256 units   14.1 ->  8.4 us     1,000 tokens, 256 units 23.9 -> 17.8 us

@@ -132,8 +132,8 @@ __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
     h.store(p);
 }
 
-// Two floats in a register pair, and the instructions on both (each rounded as
-// the single one).
+// Two floats in a register pair, and their sums (tc.cuh: products).  The compiler
+// may join a packed product and the packed sum that it feeds into one rounding.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -147,16 +147,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 __device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
 }
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 
 // Quantises a block held by 4 consecutive lanes, 8 dimensions each (lane t of
 // the four: dimensions 8 t .. + 7).  Returns this lane's word; *scale gets the
@@ -169,7 +159,7 @@ __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t* 
 #pragma unroll
     for (int i = 0; i < 8; ++i) hi = fmaxf(hi, x[i]), lo = fminf(lo, x[i]);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) bad2 = f2_fma(pair(x[i], x[i + 1]), 0, bad2);
+    for (int i = 0; i < 8; i += 2) bad2 = tc::f2_fma(pair(x[i], x[i + 1]), 0, bad2);
     float bad, bad_hi;
     unpair(bad2, bad, bad_hi);
     bad += bad_hi;

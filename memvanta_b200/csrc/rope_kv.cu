@@ -247,8 +247,8 @@ __device__ __forceinline__ void rotate8(float (&y)[8], const Held<T, 8, VEC>& pa
         if constexpr (VEC) {
 #pragma unroll
             for (int k = 0; k < 8; k += 2)
-                unpair(f2_fma(pair(y[k], y[k + 1]), pair(c[k], c[k + 1]),
-                              f2_mul(pair(o[k], o[k + 1]), pair(s[k], s[k + 1]))),
+                unpair(tc::f2_fma(pair(y[k], y[k + 1]), pair(c[k], c[k + 1]),
+                              tc::f2_mul(pair(o[k], o[k + 1]), pair(s[k], s[k + 1]))),
                        y[k], y[k + 1]);
         } else {
 #pragma unroll

@@ -402,6 +402,28 @@ def test_decode_few_and_many_units(cuda, n_seq, heads, H, hd, longest, dtype):
     assert torch.equal(got, mv.paged_attn_q4(*args))
 
 
+def test_decode_long_sums_are_rounded(cuda):
+    """The tensor cores cut their running sums; 120,000 tokens are 70 MMAs to a
+    warp.  Rounded totals every 32: half of 32 cuts of at most 2^-24 of the sum on
+    average, 9.5e-7, two factors of 22 bits, 2.4e-7, and the exponentials' 2^-22."""
+    import torch
+    H, hd, page, T = 8, 128, 128, 120_000
+    t, total = scattered([T], page, 83)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 84)
+    q = randn((1, H, hd), 85, "float32", 0.6)
+    got = mv.paged_attn_q4(q, kp, vp, ks, vs, torch.from_numpy(t).cuda(),
+                           torch.tensor([T], dtype=torch.int32, device=cuda), T).double()
+    pg = torch.from_numpy(t[0, :-(-T // page)].astype(np.int64)).cuda()
+    off = size = 0.0
+    for h in range(H):
+        k = values64(kp[pg, h], ks[pg, h]).reshape(-1, hd)[:T]
+        v = values64(vp[pg, h], vs[pg, h]).reshape(-1, hd)[:T]
+        want = torch.softmax(k @ q[0, h].double() * hd ** -0.5, 0) @ v
+        off += float(((got[0, h] - want) ** 2).sum())
+        size += float((want ** 2).sum())
+    assert (off / size) ** 0.5 <= 1.5e-6
+
+
 def test_decode_garbage_past_the_context(cuda):
     """NaN scales, wild pages and stale nibbles past ctx_len change nothing; a
     page that does not exist is left out; max_ctx cuts."""
