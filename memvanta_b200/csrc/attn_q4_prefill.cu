@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             }
             dm = __reduce_max_sync(0xffffffffu, dm);
             const bool some = __any_sync(0xffffffffu, bad);
-            const int e = max(-126, min(126, 6 - ((int)(dm >> 7) - 127)));
+            // (a tile without scales, of zeros or of missing tokens: any exponent does)
+            const int e = dm ? max(-126, min(126, 6 - ((int)(dm >> 7) - 127))) : 0;
             const float up = pow2i(e);
             if (!__all_sync(0xffffffffu,
                             tc::mbar_wait(k_empty(s), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, &g_q4_status, 47)))
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         __syncwarp();  // the exponents, too
         if (tiles) asm volatile("bar.arrive %0, 160;" ::"r"(1 + q_of) : "memory");
         const uint32_t tm = tmem + q_of * C::kCols + ((uint32_t)(warp % 4) << 21);  // this warp's 32 lanes
-        const float c_row = fmaxf(a.scale * 1.44269504088896341f * pow2i(-q_exp[q_of * kRows + m_of]), 1e-37f);
+        const float c_row = a.scale * 1.44269504088896341f * pow2i(-q_exp[q_of * kRows + m_of]);
         float m_run = -INFINITY, l = 0.0f;
         uint32_t bad = 0;  // blocks of dimensions in which this row sees values that are not finite
         bool ok = true;
@@ -575,7 +576,9 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
 #pragma unroll
             for (int j = 0; j < NT / 32; ++j) tc::tmem_ld32(ts + 32 * j, s[j]);
             tc::tmem_wait_ld();
-            const float c = c_row * k_back[i % kRing];
+            // above zero: a masked score is -inf, and -inf * 0 would be NaN.  Scores stay
+            // below 2^33 here, so a factor that small makes every one of them vanish.
+            const float c = fmaxf(c_row * k_back[i % kRing], 1e-37f);
             const int left = ctx - i * NT;  // of this row's tokens
             bool cut = left < NT;
             uint32_t msk[NT / 32];  // tokens that this row sees
