@@ -686,7 +686,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         // ---- the join, out = sum_w 2^(m_w - m) o_w / sum_w 2^(m_w - m) l_w: over the
         // CTA's warps, then over the cluster's CTAs, each of which takes a share of
         // the columns (4 dimensions of a head).  What a part without tokens holds
-        // does not count.
+        // does not count: its sum is zero.  (Its maximum is -inf, but so is that of
+        // a part whose scores are all NaN, and that one's NaN has to be seen.)
         const int h0 = at.kvh * G + at.chunk * sp.heads, nh = min(sp.heads, G - at.chunk * sp.heads);
         const int columns = nh * (HD / 4), ml_at = sp.heads * HD;  // in floats; the CTA's own after the warp's
         auto add = [](float f, const float4& x, float4& y) {
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                if (x[w].x == -INFINITY) continue;
+                if (x[w].y == 0.0f) continue;
                 const float f = ex2(x[w].x - m);
                 l = fmaf(f, x[w].y, l);
                 add(f, reinterpret_cast<const float4*>(smem + w * X::kRing)[c], y);
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                if (r >= sp.cluster || x[r].x == -INFINITY) continue;
+                if (r >= sp.cluster || x[r].y == 0.0f) continue;
                 const float f = ex2(x[r].x - m);
                 l = fmaf(f, x[r].y, l);
                 add(f, u[r], y);
@@ -778,7 +779,7 @@ __global__ void __launch_bounds__(kJoin) attn_q4_join_kernel(AttnQ4Args a, Q4Spl
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (r + i * groups >= parts || x[i].x == -INFINITY) continue;
+                if (r + i * groups >= parts || x[i].y == 0.0f) continue;  // (no tokens: the sum, as above)
                 const float m = fmaxf(top, x[i].x), e = ex2(top - m), c = ex2(x[i].x - m);
                 y[0] = fmaf(c, u[i].x, e * y[0]), y[1] = fmaf(c, u[i].y, e * y[1]);
                 y[2] = fmaf(c, u[i].z, e * y[2]), y[3] = fmaf(c, u[i].w, e * y[3]);
@@ -796,7 +797,7 @@ __global__ void __launch_bounds__(kJoin) attn_q4_join_kernel(AttnQ4Args a, Q4Spl
             float v = 0.0f, den = 0.0f, m = -INFINITY;
             for (int w = 0; w < groups; ++w) m = fmaxf(m, red[w][HD + 1]);
             for (int w = 0; w < groups; ++w) {
-                const float c = red[w][HD + 1] == -INFINITY ? 0.0f : ex2(red[w][HD + 1] - m);
+                const float c = red[w][HD] == 0.0f ? 0.0f : ex2(red[w][HD + 1] - m);
                 v = fmaf(c, red[w][i], v), den = fmaf(c, red[w][HD], den);
             }
             out[i] = from_f32<T>(den == 0.0f ? 0.0f : v / den);

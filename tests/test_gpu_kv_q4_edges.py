@@ -72,3 +72,46 @@ def test_prefill_small_queries_over_missing_tiles(cuda, dtype, hd, H, heads):
     inside = np.array([sum(min(page, max(0, c - page * p)) for p in there) for c in ctx])
     want, bound = attention64(q, kp, ks, vp, vs, t[:, there], [0] * rows, inside, page, hd ** -0.5)
     check_attention(got, want, bound)
+
+
+# ------------------------------------------------- scores that are no numbers
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("route,n,heads,H,hd,ctx", [
+    ("cluster", 2, 8, 2, 128, 700), ("runs, joined", 1, 16, 8, 128, 9000), ("runs, whole", 300, 8, 4, 64, 40),
+    ("many runs, joined", 130, 8, 8, 128, 1500)])
+def test_decode_nan_query_gives_nan(cuda, dtype, route, n, heads, H, hd, ctx):
+    """A NaN in one head's query is a NaN in all of its output, and in no other
+    head's, however the context is split."""
+    import torch
+    t, total = scattered([ctx] * n, 64, 96)
+    kp, ks, vp, vs = random_cache(total, H, 64, hd, 97)
+    q = randn((n, heads, hd), 98, dtype)
+    args = (kp, vp, ks, vs, dev(t), i32([ctx] * n), ctx)
+    clean = mv.paged_attn_q4(q, *args)
+    rows = sorted({0, n // 2, n - 1})
+    for r in rows:
+        q[r, 1, 7] = float("nan")
+    got = mv.paged_attn_q4(q, *args)
+    others = torch.tensor([r for r in range(n) if r not in rows], dtype=torch.long, device=cuda)
+    assert torch.isfinite(clean).all() and torch.equal(got[others], clean[others])
+    heads_left = [h for h in range(heads) if h != 1]
+    want, bound = attention64(q[rows], kp, ks, vp, vs, t[rows], range(len(rows)), [ctx] * len(rows), 64, hd ** -0.5)
+    assert got[rows][:, 1].isnan().all()
+    check_attention(got[rows][:, heads_left], want[:, heads_left], bound[:, heads_left])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,ctx", [(128, 1), (128, 33), (128, 705), (64, 65), (256, 17), (128, 8993), (64, 20481)])
+def test_decode_nan_key_alone_in_its_stage(cuda, dtype, hd, ctx):
+    """The last token of a context, the first of its stage, with a NaN key."""
+    import torch
+    heads, H, page = 4, 2, 16
+    t, total = scattered([ctx], page, 99)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 100)
+    ks[int(t[0, (ctx - 1) // page]), 1, (ctx - 1) % page, 0] = float("nan")
+    q = randn((1, heads, hd), 101, dtype)
+    got = mv.paged_attn_q4(q, kp, vp, ks, vs, dev(t), i32([ctx]), ctx)
+    assert got[0, 2:].isnan().all() and torch.isfinite(got[0, :2]).all()
+    chunk = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, 1]), 1, i32([ctx]), ctx)
+    assert chunk[0, 2:].isnan().all() and torch.isfinite(chunk[0, :2]).all()
