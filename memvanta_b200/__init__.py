@@ -47,7 +47,7 @@ def _t_ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_torch_module = _current = None
+_torch_module = _current = _device = None
 
 
 def _torch():
@@ -57,6 +57,16 @@ def _torch():
         import torch
         _torch_module = torch
     return _torch_module
+
+
+def _current_device() -> int:
+    """Index of the current GPU (torch.cuda.current_device() without its checks)."""
+    global _device
+    if _device is None:
+        import torch
+        torch.cuda.init()
+        _device = torch._C._cuda_getDevice
+    return _device()
 
 
 def _current_stream():
@@ -369,6 +379,17 @@ def _bad(msg: str):
     raise MemVantaError(_lib.MV_ERR_INVALID, msg)
 
 
+def _on_gpu(x, *tensors):
+    """Refuses tensors that are not all on the current GPU: the kernels would
+    read and write addresses that are none of its memory.  (0.07 us a tensor.)"""
+    at = x.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            _bad("tensors must be CUDA tensors, all of them on the current GPU")
+    if at < 0 or at != _current_device():
+        _bad("tensors must be CUDA tensors, all of them on the current GPU")
+
+
 def _heads(name: str, t, rows: int | None = None, hd: int | None = None):
     """Row and head stride of an activation tensor, checked."""
     shape, stride = t.shape, t.stride()
@@ -415,6 +436,7 @@ def rope_table(rot_dim: int, n_pos: int, theta: float = 10000.0, scaling: int = 
     if freq_factors is not None and (freq_factors.dtype != torch.float32 or not freq_factors.is_contiguous()
                                      or freq_factors.numel() != rot_dim // 2):
         _bad("freq_factors must be a contiguous float32 tensor of rot_dim / 2 elements")
+    _on_gpu(cos_t, freq_factors)
     check(load().mv_rope_table(rot_dim, n_pos, theta, scaling, factor, orig_ctx, beta_fast, beta_slow, attn_factor,
                                _t_ptr(freq_factors), _t_ptr(cos_t), _t_ptr(sin_t), _stream(stream)))
     return cos_t, sin_t
@@ -424,6 +446,7 @@ def rope_apply(x, cos_t, sin_t, pos, layout: int = ROPE_HALF, rot_dim: int | Non
     """x [rows, heads, head_dim] with the first rot_dim (default: the tables'
     width) dimensions of each head rotated by its row's position; out may be x."""
     rows, n_head, hd = x.shape
+    _on_gpu(x, cos_t, sin_t, pos, out)
     if out is None:
         import torch
         out = torch.empty((rows, n_head, hd), dtype=x.dtype, device=x.device)
@@ -491,6 +514,7 @@ def rope_kv_append(kv_type: int, q, k, v, cos_t, sin_t, pos, block_table, page: 
     """Rotates q (may be None) into q_out and k into the paged cache, and stores
     v (mv_rope_kv_append); returns q_out.  Without tables nothing is rotated."""
     rows, n_head_kv, hd = k.shape
+    _on_gpu(k, q, v, cos_t, sin_t, pos, block_table, k_pages, v_pages, k_scales, v_scales, seq, q_out)
     ks, vs = _heads("k", k), _heads("v", v, rows, hd)
     if v.shape[1] != n_head_kv or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         _bad("q, k and v must have one type, k and v the same heads")
@@ -522,6 +546,7 @@ def kv_read(kv_type: int, pages, scales, pos, block_table, page: int, n_head_kv:
     head_dim] of dtype (default float32) (mv_kv_read)."""
     import torch
     rows = pos.numel()
+    _on_gpu(pages, scales, pos, block_table, seq, out)
     if out is None:
         out = torch.empty((rows, n_head_kv, head_dim), dtype=dtype or torch.float32, device=pages.device)
     elif tuple(out.shape) != (rows, n_head_kv, head_dim) or not out.is_contiguous():
@@ -534,9 +559,10 @@ def kv_read(kv_type: int, pages, scales, pos, block_table, page: int, n_head_kv:
     return out
 
 
-def _q4_args(q, k_pages, v_pages, k_scales, v_scales, out):
+def _q4_args(q, k_pages, v_pages, k_scales, v_scales, out, *arrays):
     """Checked (type, strides, sizes) of a 4-bit attention call; pools as kv_pools shapes them."""
     rows, n_head, hd = q.shape
+    _on_gpu(q, k_pages, v_pages, k_scales, v_scales, out, *arrays)
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] * 2 != hd:
         _bad("pools must be [n_pages, n_head_kv, page, head_dim / 2], the same for k and v")
     n_pages, n_head_kv, page, _ = k_pages.shape
@@ -560,7 +586,8 @@ def paged_attn_q4(q, k_pages, v_pages, k_scales, v_scales, block_table, ctx_len,
                   out=None, stream=None):
     """Attention over a 4-bit cache, one query row per sequence: q [n_seq,
     heads, head_dim], row i sees its first ctx_len[i] tokens (mv_paged_attn_q4)."""
-    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out)
+    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out,
+                                                                       block_table, ctx_len)
     table, n_seq, max_pages = _table(block_table)
     if n_seq != q.shape[0]:
         _bad(f"the block table has {n_seq} sequences, q {q.shape[0]} rows")
@@ -575,7 +602,8 @@ def paged_attn_q4_prefill(q, k_pages, v_pages, k_scales, v_scales, block_table, 
                           max_ctx: int, scale: float = 0.0, out=None, stream=None):
     """The same for chunks of query rows: sequence s owns rows q_start[s] ..
     q_start[s + 1] of q, row r sees ctx_len[r] tokens (mv_paged_attn_q4_prefill)."""
-    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out)
+    out, ty, qr, orow, n_head, n_head_kv, hd, page, n_pages = _q4_args(q, k_pages, v_pages, k_scales, v_scales, out,
+                                                                       block_table, q_start, ctx_len)
     table, n_seq, max_pages = _table(block_table)
     check(load().mv_paged_attn_q4_prefill(ty, q.data_ptr(), qr, q.shape[0], n_head, n_head_kv, hd, k_pages.data_ptr(),
                                           v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), table, n_seq,
