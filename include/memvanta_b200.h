@@ -327,7 +327,8 @@ MV_API int mv_paged_attn_q4(int type, const void* q_dev, uint64_t q_row_stride, 
 /* The same for chunks of query rows: sequence s owns rows q_start[s] ..
  * q_start[s+1] of the n_q rows (device array of n_seq + 1, ascending from 0 to
  * n_q), at most max_q of them; row r attends to its first ctx_len[r] tokens
- * (causal: start + i + 1).  Rows of no sequence give zeros. */
+ * (causal: start + i + 1).  Rows of no sequence, and a sequence's rows past its
+ * first max_q, give zeros. */
 MV_API int mv_paged_attn_q4_prefill(int type, const void* q_dev, uint64_t q_row_stride, uint64_t n_q, uint64_t n_head,
                                     uint64_t n_head_kv, uint64_t head_dim, const void* k_pages_dev,
                                     const void* v_pages_dev, const void* k_scales_dev, const void* v_scales_dev,

@@ -27,7 +27,7 @@ namespace mvb {
 namespace {
 
 // The sequence of query row r: r itself, or by bisection of q_start (ascending);
-// -1: none.
+// -1: none, or past the max_q rows that it may have.
 __device__ __forceinline__ int seq_of_row(const AttnQ4Args& a, int r) {
     if (a.one_seq) return 0;
     if (!a.q_start) return r;
@@ -38,7 +38,7 @@ __device__ __forceinline__ int seq_of_row(const AttnQ4Args& a, int r) {
         if (a.q_start[mid] <= r) lo = mid;
         else hi = mid - 1;
     }
-    return lo;
+    return (uint64_t)(r - a.q_start[lo]) < a.max_q ? lo : -1;
 }
 
 // ------------------------------------------------------------- primitives

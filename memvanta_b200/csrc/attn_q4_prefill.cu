@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
     rest /= p.chunks;
     const int kvh = rest % H, seq = rest / H;
     const int64_t seq0 = a.one_seq ? 0 : min(max(a.q_start[seq], 0), (int)a.n_q);
-    const int64_t seq1 = a.one_seq ? (int64_t)a.n_q : min(max(a.q_start[seq + 1], 0), (int)a.n_q);
+    const int64_t end = a.one_seq ? (int64_t)a.n_q : min(max(a.q_start[seq + 1], 0), (int)a.n_q);
+    const int64_t seq1 = min(end, seq0 + (int64_t)a.max_q);
     const int64_t row0 = seq0 + (int64_t)qt * NQ * p.rpt;
     const int h0 = kvh * G + chunk * p.heads, nh = min(p.heads, G - chunk * p.heads);
     if (qt == p.q_tiles - 1) {  // rows of no chunk, and past max_q, are zeros
@@ -183,9 +184,9 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                 for (int k = threadIdx.x; k < nh * HD; k += blockDim.x)
                     static_cast<T*>(a.out)[r * (int64_t)a.out_stride + (int64_t)h0 * HD + k] = T(0.0f);
         };
-        zeros(seq0 + (int64_t)p.q_tiles * NQ * p.rpt, seq1);
+        zeros(seq1, end);
         if (seq == 0) zeros(0, seq0);
-        if (seq == (int)a.n_seq - 1) zeros(max(seq0, seq1), (int64_t)a.n_q);
+        if (seq == (int)a.n_seq - 1) zeros(max(seq0, end), (int64_t)a.n_q);
     }
     if (row0 >= seq1) return;
 

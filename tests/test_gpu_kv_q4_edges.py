@@ -115,3 +115,25 @@ def test_decode_nan_key_alone_in_its_stage(cuda, dtype, hd, ctx):
     assert got[0, 2:].isnan().all() and torch.isfinite(got[0, :2]).all()
     chunk = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, 1]), 1, i32([ctx]), ctx)
     assert chunk[0, 2:].isnan().all() and torch.isfinite(chunk[0, :2]).all()
+
+
+# ------------------------------------------------------------- rows and routes
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,max_q", [(300, 200), (300, 100), (20, 7)])
+def test_prefill_rows_past_max_q_are_zeros(cuda, dtype, rows, max_q):
+    """In large chunks and in small ones."""
+    import torch
+    heads, H, hd, page = 8, 8, 128, 16
+    chunks = [rows, 3, rows]
+    starts = np.concatenate([[0], np.cumsum(chunks)]).astype(np.int32)
+    ctx = np.concatenate([np.arange(1, n + 1) for n in chunks]).astype(np.int32)
+    t, total = scattered(chunks, page, 102)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 103)
+    q = randn((len(ctx), heads, hd), 104, dtype)
+    seq = np.repeat(np.arange(3), chunks)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), dev(starts), max_q, dev(ctx), rows)
+    want, bound = attention64(q, kp, ks, vp, vs, t, seq, ctx, page, hd ** -0.5)
+    past = dev(np.arange(len(ctx)) - starts[seq] >= max_q)
+    assert not got[past].any()
+    check_attention(got[~past], want[~past], bound[~past])
