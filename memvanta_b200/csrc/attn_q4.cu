@@ -913,14 +913,22 @@ cudaError_t decode_of(int type, const AttnQ4Args& a, cudaStream_t s, uint64_t* n
 }
 
 // Chunks go row by row through the kernel above while they are small: a row and
-// kv head costs it 54 ps a token (head_dim 128: 57 us for 131,071 tokens of 8),
-// whereas a wave of the tensor-core kernel's CTAs takes 19 ns a token (fp32
-// queries 28 ns) however few of its 128 rows are used -- 350 or 520 times that.
+// kv head costs it 46 to 57 ps a token (head_dim 128, fp32), whereas a wave of the
+// tensor-core kernel's CTAs takes 25 ns a token however few of its 128 rows are
+// used -- as much as 550 rows.  Measured by head_dim 64, 128, 256: 820, 550, 770 rows
+// (fp32 queries), 640, 415, 440 (half precision).  The bounds lie below all of them,
+// since a causal chunk's first rows are cheap for both and its tiles are not.
+// Only the tiles that hold rows count, each sequence's last one part empty; a CTA
+// without rows leaves its SM after 1.1 us, a wave's 25 ns for 44 tokens.  One chunk of
+// 2,048 rows and 63 single rows after 700 tokens, 32 heads x 128: fp32 775 us (row by
+// row 5,085), 32 heads / 8 bf16 290 us (1,259).
 bool rows_one_by_one(int type, const AttnQ4Args& a) {
     const uint64_t G = a.n_head / a.n_head_kv, heads = type == kTypeF32 && G <= 4 ? 4 : 8;
-    const uint64_t rpt = 128 / std::min<uint64_t>(G, 128);
-    const uint64_t ctas = a.n_seq * a.n_head_kv * ((G + 127) / 128) * ((a.max_q + rpt - 1) / rpt);
-    return a.n_q * a.n_head_kv * ((G + heads - 1) / heads) < (type == kTypeF32 ? 520 : 350) * ((ctas + 147) / 148);
+    const uint64_t rpt = 128 / std::min<uint64_t>(G, 128), units = a.n_head_kv * ((G + 127) / 128);
+    const uint64_t ctas = prefill_tiles(a, rpt) * units, grid = a.n_seq * ((a.max_q + rpt - 1) / rpt) * units;
+    const uint64_t wave = type == kTypeF32 ? 520 : 350, empty = (grid - ctas) / 148;
+    return a.n_q * a.n_head_kv * ((G + heads - 1) / heads) <
+           wave * ((ctas + 147) / 148) + wave * 44 * empty / std::max<uint64_t>(44, a.max_ctx);
 }
 
 }  // namespace

@@ -717,8 +717,7 @@ template <class T>
 cudaError_t prefill_of(const PfArgs& p, cudaStream_t s) {
     // two query tiles to a CTA share each expanded tile of the cache, where that
     // still gives every SM a CTA
-    const uint64_t units = p.a.n_seq * p.a.n_head_kv * (uint64_t)p.chunks;
-    const bool two = ((p.a.max_q + (uint64_t)(2 * p.rpt) - 1) / (uint64_t)(2 * p.rpt)) * units >= 148;
+    const bool two = prefill_tiles(p.a, 2 * (uint64_t)p.rpt) * p.a.n_head_kv * (uint64_t)p.chunks >= 148;
     if constexpr (sizeof(T) == 2) {  // (fp32: tensor memory holds one)
         if (two && p.a.hd == 64) return launch_prefill<T, 64, 2>(p, s);
         if (two && p.a.hd == 128) return launch_prefill<T, 128, 2>(p, s);

@@ -247,6 +247,12 @@ uint64_t attn_q4_workspace(int type, const AttnQ4Args& a);
 cudaError_t attn_q4(int type, const AttnQ4Args& a, cudaStream_t s);
 // attn_q4_prefill.cu : the same for chunks (q_start, one_seq), on tcgen05
 cudaError_t attn_q4_prefill(int type, const AttnQ4Args& a, cudaStream_t s);
+// Tiles of `rows` query rows that hold any, at most: sequences of max_q rows each, or
+// n_q rows in all and a part of a tile more for each sequence.
+inline uint64_t prefill_tiles(const AttnQ4Args& a, uint64_t rows) {
+    const uint64_t each = a.n_seq * ((a.max_q + rows - 1) / rows), all = a.n_q / rows + a.n_seq;
+    return each < all ? each : all;
+}
 cudaError_t q4_status_take(int* status);
 
 uint64_t attn_smem_bytes(uint64_t hd, uint64_t max_ctx, uint64_t max_pages, int kv_type);

@@ -137,3 +137,25 @@ def test_prefill_rows_past_max_q_are_zeros(cuda, dtype, rows, max_q):
     past = dev(np.arange(len(ctx)) - starts[seq] >= max_q)
     assert not got[past].any()
     check_attention(got[~past], want[~past], bound[~past])
+
+
+def test_a_long_chunk_beside_single_rows_keeps_its_bits(cuda):
+    """A chunk that is large enough for the tensor cores goes through them beside
+    63 sequences of a single row too: its rows' bits are those of the chunk alone,
+    where the row-by-row kernel's differ."""
+    import torch
+    heads, H, hd, page, rows, n = 8, 8, 128, 32, 600, 64
+    need = [rows] + [50 + i for i in range(1, n)]
+    t, total = scattered(need, page, 105)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 106)
+    q = randn((rows + n - 1, heads, hd), 107)
+    ctx = np.r_[np.arange(1, rows + 1), need[1:]].astype(np.int32)
+    starts = np.r_[0, rows + np.arange(n)].astype(np.int32)
+    alone = mv.paged_attn_q4_prefill(q[:rows], kp, vp, ks, vs, dev(t[:1]), i32([0, rows]), rows, dev(ctx[:rows]), rows)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), dev(starts), rows, dev(ctx), rows)
+    by_row = mv.paged_attn_q4(q[:rows], kp, vp, ks, vs, dev(np.repeat(t[:1], rows, 0)), dev(ctx[:rows]), rows)
+    assert not torch.equal(by_row, alone)
+    assert torch.equal(got[:rows], alone)
+    seq = np.r_[np.zeros(rows, int), np.arange(1, n)]
+    want, bound = attention64(q, kp, ks, vp, vs, t, seq, ctx, page, hd ** -0.5)
+    check_attention(got, want, bound)
