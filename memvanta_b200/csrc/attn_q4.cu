@@ -113,8 +113,10 @@ struct Q4Tile {
     static constexpr int kScale = TT * NB * 2;
     static constexpr int kBytes = 2 * 2048 + 2 * kScale;  // K, V, K scales, V scales
     static constexpr int kRing = kStages * kBytes;
-    static constexpr int kTotal = HD * 8 * 4;  // a warp's outputs so far: 16 x 8 per 16 dimensions, both parts
-    static constexpr int kFlush = 32 / NJ;     // stages between their sums
+    // a warp's outputs so far, 16 x 8 per 16 dimensions (both parts), and the references that they are on
+    static constexpr int kTotal = HD * 8 * 4 + 32 * 4;
+    static constexpr int kFlush = 32 / NJ;  // stages between their sums, fp32 queries
+    static constexpr int kRun = 1024 / NJ;  // and half precision
     // unit u of token row r sits at u ^ swz(r): the fragment loads are then
     // free of bank conflicts (8 rows x 16 bytes, or 4 rows 2 apart)
     static __device__ __forceinline__ int swz(int r) { return (r >> (U == 8 ? 0 : U == 4 ? 1 : 2)) & (U - 1); }
@@ -404,9 +406,35 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
     // moves, the outputs are added, rounded, to totals in shared memory and start
     // from zero.  131,071 tokens: relative error 1.6e-6 to 2.3e-6 without, 4.5e-7 to
     // 8.8e-7 so (every 16: 3.6e-7 to 5.0e-7), for 59.5 us instead of 56.0.
+    // Half precision: every 1,024 MMAs, outside the loop over the stages (inside it, as
+    // above, 64 x 2,000 tokens of 8 kv heads took 80 us for 58: registers).  Outputs of
+    // values of one sign after 262,144 tokens in one warp: 1.1e-3 short without, four
+    // times fp16's rounding, 2.7e-5 so.
     float4* total = reinterpret_cast<float4*>(smem + kWarps * X::kRing + warp * X::kTotal) + lane;
+    float* total_m = reinterpret_cast<float*>(total - lane + HD * 2) + lane;
     bool held = false;  // something is in the totals
     float m_run = -INFINITY, l_run = 0.0f;
+    auto add_total = [&] {  // to the outputs, on their reference (fp32 queries' totals are always on it)
+        if ((CL && !kTwo) || !held) return;
+        uint64_t aa = 0;
+        if constexpr (!kTwo) {
+            const float alpha = m_run == -INFINITY ? 0.0f : ex2(*total_m - m_run);
+            aa = pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float(&x)[4] = o[b][m];
+                const float4 y = total[(2 * b + m) * 32];
+                if constexpr (kTwo) {
+                    x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+                } else {
+                    unpair(tc::f2_fma(pair(y.x, y.y), aa, pair(x[0], x[1])), x[0], x[1]);
+                    unpair(tc::f2_fma(pair(y.z, y.w), aa, pair(x[2], x[3])), x[2], x[3]);
+                }
+            }
+    };
     uint32_t off = 0, refill = (kStages - 1) * X::kBytes;  // of the stage computed, and of the one copied into
     if (CL && !count && lane < sp.heads)  // nothing of this warp's counts
         *reinterpret_cast<float2*>(ring + sp.heads * HD * 4 + lane * 8) = make_float2(-INFINITY, 0.0f);
@@ -460,167 +488,172 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         m_run = -INFINITY;
         l_run = 0.0f;
         held = false;
-        for (; at.stage < end; ++at.stage, ++n) {
-            cp_async_wait<kStages - 2>();
-            __syncwarp();
-            const uint8_t* kt = ring + off;
-            const uint8_t* vt = kt + 2048;
-            const uint8_t* ksc = kt + 4096;
-            const uint8_t* vsc = ksc + X::kScale;
+        for (int stop = kTwo || CL ? end : min(end, from + X::kRun);; stop = min(end, stop + X::kRun)) {
+            for (; at.stage < stop; ++at.stage, ++n) {
+                cp_async_wait<kStages - 2>();
+                __syncwarp();
+                const uint8_t* kt = ring + off;
+                const uint8_t* vt = kt + 2048;
+                const uint8_t* ksc = kt + 4096;
+                const uint8_t* vsc = ksc + X::kScale;
 
-            // ---- scores
-            float sc[NJ][2];
+                // ---- scores
+                float sc[NJ][2];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                uint32_t w[NB], d[NB];
-                load_words<HD>(w, kt, 8 * j + g, t);
-                load_scales<HD>(d, ksc, 8 * j + 2 * t);
-                uint64_t sum = 0;  // two zeros
+                for (int j = 0; j < NJ; ++j) {
+                    uint32_t w[NB], d[NB];
+                    load_words<HD>(w, kt, 8 * j + g, t);
+                    load_scales<HD>(d, ksc, 8 * j + 2 * t);
+                    uint64_t sum = 0;  // two zeros
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int b = 0; b < NB; ++b) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t x = k ? w[b] >> 8 : w[b];
-                        uint32_t qf[4];
-                        if constexpr (kTwo) {
-                            qf[0] = qa[b][k][0], qf[1] = qa[b][k][1], qf[2] = qa[b][k][2], qf[3] = qa[b][k][3];
-                        } else {
-                            qf[0] = qa[b][k][0], qf[1] = 0, qf[2] = qa[b][k][1], qf[3] = 0;
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t x = k ? w[b] >> 8 : w[b];
+                            uint32_t qf[4];
+                            if constexpr (kTwo) {
+                                qf[0] = qa[b][k][0], qf[1] = qa[b][k][1], qf[2] = qa[b][k][2], qf[3] = qa[b][k][3];
+                            } else {
+                                qf[0] = qa[b][k][0], qf[1] = 0, qf[2] = qa[b][k][1], qf[3] = 0;
+                            }
+                            mma16816(c, qf, nib_lo(x), nib_hi(x), c);
                         }
-                        mma16816(c, qf, nib_lo(x), nib_hi(x), c);
+                        const uint64_t dd = pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b));
+                        uint64_t cc = pair(c[0], c[1]);
+                        if constexpr (kTwo) cc = f2_add(cc, pair(c[2], c[3]));
+                        sum = tc::f2_fma(cc, dd, sum);
                     }
-                    const uint64_t dd = pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b));
-                    uint64_t cc = pair(c[0], c[1]);
-                    if constexpr (kTwo) cc = f2_add(cc, pair(c[2], c[3]));
-                    sum = tc::f2_fma(cc, dd, sum);
+                    unpair(sum, sc[j][0], sc[j][1]);
                 }
-                unpair(sum, sc[j][0], sc[j][1]);
-            }
-            // tokens that do not exist
+                // tokens that do not exist
 #pragma unroll
-            for (int i = 0; i < LT; ++i) {
-                const uint32_t v = valid[0][i], full = TT >= 32 ? 0xffffffffu : (1u << (TT & 31)) - 1u;
-                if (v != full) {
+                for (int i = 0; i < LT; ++i) {
+                    const uint32_t v = valid[0][i], full = TT >= 32 ? 0xffffffffu : (1u << (TT & 31)) - 1u;
+                    if (v != full) {
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-                        if (j / 4 == i) {
-                            const uint32_t k = v >> (8 * (j % 4) + 2 * t);
-                            if (!(k & 1u)) sc[j][0] = -INFINITY;
-                            if (!(k & 2u)) sc[j][1] = -INFINITY;
-                        }
+                        for (int j = 0; j < NJ; ++j)
+                            if (j / 4 == i) {
+                                const uint32_t k = v >> (8 * (j % 4) + 2 * t);
+                                if (!(k & 1u)) sc[j][0] = -INFINITY;
+                                if (!(k & 2u)) sc[j][1] = -INFINITY;
+                            }
+                    }
                 }
-            }
-            // ---- running maximum, weights
-            float mx = sc[0][0];
+                // ---- running maximum, weights
+                float mx = sc[0][0];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(sc[j][0], sc[j][1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // The reference m follows the maximum only once that is 2^8 above it:
-            // weights up to 2^8 do no harm, and the outputs are seldom rescaled.
-            mx *= c_h;
-            const bool sum = kTwo && at.stage != from && (at.stage - from) % X::kFlush == 0;
-            if (sum || __any_sync(0xffffffffu, mx > m_run + 8.0f)) {
-                const float m_new = fmaxf(m_run, mx), alpha = m_new == -INFINITY ? 0.0f : ex2(m_run - m_new);
-                l_run *= alpha;
-                const uint64_t aa =
-                pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
+                for (int j = 0; j < NJ; ++j) mx = fmaxf(mx, fmaxf(sc[j][0], sc[j][1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // The reference m follows the maximum only once that is 2^8 above it:
+                // weights up to 2^8 do no harm, and the outputs are seldom rescaled.
+                mx *= c_h;
+                const bool sum = kTwo && at.stage != from && (at.stage - from) % X::kFlush == 0;
+                if (sum || __any_sync(0xffffffffu, mx > m_run + 8.0f)) {
+                    const float m_new = fmaxf(m_run, mx), alpha = m_new == -INFINITY ? 0.0f : ex2(m_run - m_new);
+                    l_run *= alpha;
+                    const uint64_t aa =
+                    pair(__shfl_sync(0xffffffffu, alpha, 8 * t), __shfl_sync(0xffffffffu, alpha, 8 * t + 4));
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        float(&x)[4] = o[b][m];
-                        if (kTwo && at.stage == from) continue;  // zeros
-                        uint64_t u = pair(x[0], x[1]), v = pair(x[2], x[3]);
-                        if constexpr (kTwo) {
-                            if (held) {
-                                const float4 y = total[(2 * b + m) * 32];
-                                u = f2_add(u, pair(y.x, y.y)), v = f2_add(v, pair(y.z, y.w));
+                        for (int m = 0; m < 2; ++m) {
+                            float(&x)[4] = o[b][m];
+                            if (kTwo && at.stage == from) continue;  // zeros
+                            uint64_t u = pair(x[0], x[1]), v = pair(x[2], x[3]);
+                            if constexpr (kTwo) {
+                                if (held) {
+                                    const float4 y = total[(2 * b + m) * 32];
+                                    u = f2_add(u, pair(y.x, y.y)), v = f2_add(v, pair(y.z, y.w));
+                                }
+                            }
+                            unpair(tc::f2_mul(u, aa), x[0], x[1]);
+                            unpair(tc::f2_mul(v, aa), x[2], x[3]);
+                            if constexpr (kTwo) {
+                                total[(2 * b + m) * 32] = make_float4(x[0], x[1], x[2], x[3]);
+                                x[0] = x[1] = x[2] = x[3] = 0.0f;
                             }
                         }
-                        unpair(tc::f2_mul(u, aa), x[0], x[1]);
-                        unpair(tc::f2_mul(v, aa), x[2], x[3]);
-                        if constexpr (kTwo) {
-                            total[(2 * b + m) * 32] = make_float4(x[0], x[1], x[2], x[3]);
-                            x[0] = x[1] = x[2] = x[3] = 0.0f;
-                        }
-                    }
-                held = at.stage != from;
-                m_run = m_new;
-            }
-            const float m_use = m_run == -INFINITY ? 0.0f : m_run;
-            // ---- outputs, 8 tokens at a time
-            const int half = (g & 1) * 16;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                float p[2];
-                uint32_t d[NB], w[2][NB];
-                load_scales<HD>(d, vsc, 8 * j + 2 * t);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
-                    l_run += p[i];
-                    if constexpr (!kTwo) p[i] *= kCut;
-                    load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
+                    if constexpr (kTwo) held = at.stage != from;
+                    m_run = m_new;
                 }
-                const uint64_t pp = pair(p[0], p[1]);
+                const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+                // ---- outputs, 8 tokens at a time
+                const int half = (g & 1) * 16;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float v[2];
-                    const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
-                    unpair(vv, v[0], v[1]);
-                    const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
-                    float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
-                    values2<0>(x0, bias0, f0[0], f0[1]);
-                    values2<0>(x1, bias0, f0[2], f0[3]);
-                    values2<2>(x0, bias1, f1[0], f1[1]);
-                    values2<2>(x1, bias1, f1[2], f1[3]);
-                    if constexpr (PACK) {
-                        // columns 0..3: v, cut to 11 bits by the MMA; 4..7: v less its first 11 bits
-                        const uint64_t cut = pair(-__uint_as_float(__float_as_uint(v[0]) & first),
-                                                  -__uint_as_float(__float_as_uint(v[1]) & first));
-                        unpair(f2_add(vv, cut), v[0], v[1]);
+                for (int j = 0; j < NJ; ++j) {
+                    float p[2];
+                    uint32_t d[NB], w[2][NB];
+                    load_scales<HD>(d, vsc, 8 * j + 2 * t);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
+                        l_run += p[i];
+                        if constexpr (!kTwo) p[i] *= kCut;
+                        load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
                     }
-                    mma1688(o[b][0], f0, v[0], v[1]);
-                    mma1688(o[b][1], f1, v[0], v[1]);
-                    if constexpr (kTwo && !PACK) {
+                    const uint64_t pp = pair(p[0], p[1]);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
+                    for (int b = 0; b < NB; ++b) {
+                        float v[2];
+                        const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
+                        unpair(vv, v[0], v[1]);
+                        const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
+                        float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
+                        values2<0>(x0, bias0, f0[0], f0[1]);
+                        values2<0>(x1, bias0, f0[2], f0[3]);
+                        values2<2>(x0, bias1, f1[0], f1[1]);
+                        values2<2>(x1, bias1, f1[2], f1[3]);
+                        if constexpr (PACK) {
+                            // columns 0..3: v, cut to 11 bits by the MMA; 4..7: v less its first 11 bits
+                            const uint64_t cut = pair(-__uint_as_float(__float_as_uint(v[0]) & first),
+                                                      -__uint_as_float(__float_as_uint(v[1]) & first));
+                            unpair(f2_add(vv, cut), v[0], v[1]);
+                        }
                         mma1688(o[b][0], f0, v[0], v[1]);
                         mma1688(o[b][1], f1, v[0], v[1]);
+                        if constexpr (kTwo && !PACK) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xffffe000u);
+                            mma1688(o[b][0], f0, v[0], v[1]);
+                            mma1688(o[b][1], f1, v[0], v[1]);
+                        }
                     }
                 }
-            }
-            // ---- the next copies, into the stage used before this one
-            __syncwarp();
+                // ---- the next copies, into the stage used before this one
+                __syncwarp();
 #pragma unroll
-            for (int k = 0; k + 1 < kStages; ++k)
+                for (int k = 0; k + 1 < kStages; ++k)
 #pragma unroll
-                for (int i = 0; i < LT; ++i) valid[k][i] = valid[k + 1][i];
-            if (left > 0) {
-                issue(ring_s + refill, kStages - 2);
-                if (--left) {
-                    if (++ahead.stage == ahead.stages) next_unit(ahead), new_unit();
-                    look_up();
+                    for (int i = 0; i < LT; ++i) valid[k][i] = valid[k + 1][i];
+                if (left > 0) {
+                    issue(ring_s + refill, kStages - 2);
+                    if (--left) {
+                        if (++ahead.stage == ahead.stages) next_unit(ahead), new_unit();
+                        look_up();
+                    }
                 }
+                cp_async_commit();
+                refill = off;
+                off = off + X::kBytes == X::kRing ? 0 : off + X::kBytes;
             }
-            cp_async_commit();
-            refill = off;
-            off = off + X::kBytes == X::kRing ? 0 : off + X::kBytes;
+            if (kTwo || CL || stop == end) break;
+            add_total();
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    total[(2 * b + m) * 32] = make_float4(o[b][m][0], o[b][m][1], o[b][m][2], o[b][m][3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[b][m][i] = 0.0f;
+                }
+            *total_m = m_run;
+            held = true;
         }
 
         // ---- the unit's end, or the run's
-        if constexpr (kTwo) {
-            if (held)
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const float4 y = total[(2 * b + m) * 32];
-                        o[b][m][0] += y.x, o[b][m][1] += y.y, o[b][m][2] += y.z, o[b][m][3] += y.w;
-                    }
-        }
+        add_total();
         const bool done = at.stage == at.stages;
         const bool whole = !CL && done && from == 0;
         float l = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
@@ -819,7 +852,7 @@ template <class T, int HD, bool PACK>
 cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     using X = Q4Tile<HD>;
     constexpr int kHeads = PACK ? 4 : 8;
-    const int smem = kWarps * (X::kRing + (sizeof(T) == 4 ? X::kTotal : 0));
+    const int smem = kWarps * (X::kRing + X::kTotal);
     auto kernel = attn_q4_decode_kernel<T, HD, PACK, false>;
     ensure_smem_attr(kernel, smem);
     static const uint64_t slots = resident_ctas(reinterpret_cast<const void*>(kernel), kWarps * 32, smem);
@@ -854,6 +887,7 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
             return cudaSuccess;
         }
         sp.cluster = (int)cluster;
+        const int smem = kWarps * (X::kRing + (sizeof(T) == 4 ? X::kTotal : 0));
         auto one = attn_q4_decode_kernel<T, HD, PACK, true>;
         ensure_smem_attr(one, smem);
         cudaLaunchConfig_t cfg{};

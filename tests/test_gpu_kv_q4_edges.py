@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import memvanta_b200 as mv
-from test_gpu_kv_q4 import attention64, check_attention, randn, random_cache, scattered
+from test_gpu_kv_q4 import attention64, check_attention, randn, random_cache, scattered, values64
 
 pytestmark = pytest.mark.gpu
 TYPES = ["float32", "float16", "bfloat16"]
@@ -159,3 +159,58 @@ def test_a_long_chunk_beside_single_rows_keeps_its_bits(cuda):
     seq = np.r_[np.zeros(rows, int), np.arange(1, n)]
     want, bound = attention64(q, kp, ks, vp, vs, t, seq, ctx, page, hd ** -0.5)
     check_attention(got, want, bound)
+
+
+# ------------------------------------------------- sums over long contexts
+#
+# Values of one sign, so that an output is a sum that only grows, and its error
+# of one direction shows in the mean over many outputs, where the rounding of
+# the outputs does not.  The tensor cores take up to 1e-7 of such a running sum
+# off at every MMA: 1e-3 after 262,144 tokens, several units in the last place of
+# fp16.  With a rounded total every 1,000 MMAs half of 1e-4 is left on average.
+
+# Keys of one scale: scores of a standard deviation of about 1, so that an output
+# is a sum over many tokens.
+
+def long_cache(hd, H, T, page, seed):
+    t, total = scattered([T], page, seed)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, seed + 1)
+    return t, kp, ks.fill_(0.4), vp, vs
+
+
+def one_sided(*args):
+    t, kp, ks, vp, vs = long_cache(*args)
+    return t, kp, ks, vp | 0x88, vs.abs()  # nibbles 8 .. 15: values of 0 to 7 scales
+
+
+def mean_off(got, q, ctx, t, kp, ks, vp, vs, page):
+    """Mean over the outputs of (got - want) / want; rows of one sequence."""
+    import torch
+    rows, heads, hd = q.shape
+    H, T = kp.shape[1], int(max(ctx))
+    pg = dev(t[0, :-(-T // page)].astype(np.int64))
+    past = torch.arange(T, device="cuda") >= i32(list(ctx))[:, None]
+    off = []
+    for h in range(heads):
+        g = h // (heads // H)
+        k = values64(kp[pg, g], ks[pg, g]).reshape(-1, hd)[:T]
+        v = values64(vp[pg, g], vs[pg, g]).reshape(-1, hd)[:T]
+        s = (q[:, h].double() @ k.T * hd ** -0.5).masked_fill(past, -float("inf"))
+        want = torch.softmax(s, -1) @ v
+        off.append(((got[:, h].double() - want) / want).mean())
+    return float(torch.stack(off).mean())
+
+
+@pytest.mark.parametrize("dtype,heads,hd", [("float16", 8, 128), ("float16", 8, 64), ("bfloat16", 2, 128),
+                                            ("float16", 2, 256)])
+def test_decode_long_half_sums_are_rounded(cuda, dtype, heads, hd):
+    """As many units as the GPU holds warps, and more, so that one warp walks
+    262,144 tokens: 32,768 MMAs."""
+    import torch
+    H, page, T, n = heads // 2, 128, 262_144, 2000 // (heads // 2)
+    t, kp, ks, vp, vs = one_sided(hd, H, T, page, 108)
+    q = randn((n, heads, hd), 110, dtype, 0.5)
+    got = mv.paged_attn_q4(q, kp, vp, ks, vs, dev(np.repeat(t, n, 0)), i32([T] * n), T)
+    some = list(range(0, n, n // 50))
+    noise = 1e-5 if dtype == "float16" else 4e-5  # of the outputs' rounding, over 50 x heads x hd outputs
+    assert abs(mean_off(got[some], q[some], [T] * len(some), t, kp, ks, vp, vs, page)) <= 5e-5 + noise
