@@ -18,6 +18,7 @@
 
 #include <algorithm>
 
+#include "common.cuh"
 #include "kernels.cuh"
 #include "kv_q4.cuh"
 #include "tc.cuh"
@@ -909,9 +910,8 @@ cudaError_t launch_decode(const AttnQ4Args& a, cudaStream_t s, uint64_t* need) {
     }
     uint8_t* scratch = static_cast<uint8_t*>(a.workspace);
     if (!scratch) {
-        keep_pool_memory();
         const uint64_t bytes = parts + joins * sizeof(int4);
-        if (cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&scratch), bytes, s)) return e;
+        if (cudaError_t e = scratch_alloc(reinterpret_cast<void**>(&scratch), bytes, s)) return e;
     }
     sp.scratch = reinterpret_cast<float*>(scratch);
     sp.joins = reinterpret_cast<int4*>(scratch + parts);

@@ -12,7 +12,6 @@
 #include <string>
 
 #include "../../include/memvanta_b200.h"
-#include "common.cuh"
 #include "kernels.cuh"
 #include "weights.cuh"
 
@@ -91,6 +90,17 @@ struct HostCallBuffers {
 HostCallBuffers& host_buffers() {
     static thread_local HostCallBuffers b;
     return b;
+}
+
+// Stream-ordered scratch (cudaMallocAsync) comes from the device's default
+// pool; keep freed blocks in the pool instead of returning them to the driver
+// at every synchronisation.
+void keep_pool_memory(int device) {
+    cudaMemPool_t pool;
+    if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
+        uint64_t threshold = UINT64_MAX;
+        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
+    }
 }
 
 int check_weight(const mv_weight_s* w) {
@@ -222,7 +232,7 @@ MV_API int mv_init(int device) {
     if (major != 10)
         return fail(MV_ERR_UNSUPPORTED, "memvanta_b200 is built for sm_100a; device has compute capability " +
                                             std::to_string(major) + ".x");
-    mvb::keep_pool_memory();
+    keep_pool_memory(device);
     return MV_OK;
 }
 

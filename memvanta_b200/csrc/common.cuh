@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <map>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -25,21 +26,36 @@ inline void ensure_smem_attr(Kernel* k, int bytes) {
     done.insert(key);
 }
 
-// Stream-ordered scratch (cudaMallocAsync) comes from the current device's
-// default pool; keep freed blocks in the pool instead of returning them to the
-// driver at every synchronisation.  Set once per device.
-inline void keep_pool_memory() {
+// Stream-ordered scratch on the current device, freed with cudaFreeAsync.  It comes
+// from a pool of the library's own, whose freed blocks stay in it: the device's
+// default pool is the process's, and only mv_init sets it up.  (The pool is made by
+// the first call, which may be inside a capture.)
+inline cudaError_t scratch_alloc(void** p, uint64_t bytes, cudaStream_t s) {
     static std::mutex mu;
-    static std::set<int> done;
+    static std::map<int, cudaMemPool_t> pools;
     int dev = 0;
     cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    if (!done.insert(dev).second) return;
     cudaMemPool_t pool;
-    if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess) {
-        uint64_t threshold = UINT64_MAX;
-        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        auto at = pools.find(dev);
+        if (at == pools.end()) {
+            cudaMemPoolProps props{};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = dev;
+            uint64_t threshold = UINT64_MAX;
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            cudaError_t e = cudaMemPoolCreate(&pool, &props);
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &threshold);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return e;
+            at = pools.emplace(dev, pool).first;
+        }
+        pool = at->second;
     }
+    return cudaMallocFromPoolAsync(p, bytes, pool, s);
 }
 
 // ------------------------------------------------- programmatic launches

@@ -214,3 +214,45 @@ def test_decode_long_half_sums_are_rounded(cuda, dtype, heads, hd):
     some = list(range(0, n, n // 50))
     noise = 1e-5 if dtype == "float16" else 4e-5  # of the outputs' rounding, over 50 x heads x hd outputs
     assert abs(mean_off(got[some], q[some], [T] * len(some), t, kp, ks, vp, vs, page)) <= 5e-5 + noise
+
+
+# ------------------------------------------------------------------ scratch
+
+@pytest.mark.parametrize("how", ["called", "captured first"])
+def test_scratch_leaves_the_default_pool_alone(cuda, how):
+    """A process that never called mv.init: an attention call that takes scratch
+    leaves the device's default memory pool as the process had it, and may be the
+    first call of all inside a graph capture."""
+    import subprocess
+    import sys
+    code = """
+import sys
+import torch
+from cuda.bindings import runtime as rt
+import memvanta_b200 as mv
+how, attr = sys.argv[1], rt.cudaMemPoolAttr.cudaMemPoolAttrReleaseThreshold
+torch.cuda.init()
+err, pool = rt.cudaDeviceGetDefaultMemPool(0)
+threshold = lambda: int(rt.cudaMemPoolGetAttribute(pool, attr)[1])
+before = threshold()
+T, H, hd = 20000, 8, 128
+kp, vp, ks, vs = mv.kv_pools(mv.KV_Q4_0, -(-T // 16), 16, H, hd)
+kp.random_(0, 256), vp.random_(0, 256), ks.fill_(0.1), vs.fill_(0.1)
+q = torch.randn((1, H, hd), device="cuda")
+args = (q, kp, vp, ks, vs, torch.arange(kp.shape[0], dtype=torch.int32, device="cuda")[None],
+        torch.tensor([T], dtype=torch.int32, device="cuda"), T)
+torch.cuda.synchronize()
+if how == "called":
+    got = mv.paged_attn_q4(*args)
+else:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = mv.paged_attn_q4(*args)
+    g.replay()
+torch.cuda.synchronize()
+assert torch.equal(got, mv.paged_attn_q4(*args)) and got.abs().sum() > 0
+assert threshold() == before, (threshold(), before)
+"""
+    done = subprocess.run([sys.executable, "-c", code, how], cwd=__file__.rsplit("/tests/", 1)[0], timeout=300,
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
