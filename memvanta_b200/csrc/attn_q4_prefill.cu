@@ -23,7 +23,8 @@
 // from zero and are added to the total, rounded, by the softmax warps.
 // A half-precision query is one part, and so are its weights, cut to 11 bits
 // by the tensor core, with 1 + 2^-11 0.72 on them for what that takes off on
-// average (mantissas being log-uniform).
+// average (mantissas being log-uniform).  Its outputs are summed by the tensor core
+// for kRunTokens tokens at a time.
 // A masked weight is 0, and 0 times a value that is not finite would not be: such
 // value blocks enter as zeros, and the rows that see one get NaN in its
 // dimensions at the end.
@@ -79,12 +80,19 @@ constexpr int kRows = 128;  // of a query tile: TMEM lanes
 // (measured: they come out 1.0e-6 short, of 1.2e-6 in all).
 constexpr float kSumCut = 1.0f + 1.0f / 1048576;
 constexpr float kCutLog2 = 5.0811e-4f;  // log2(kCut)
+// Half-precision queries: tokens between rounded totals of the outputs, in scratch
+// (tensor memory is full).  Outputs of values of one sign after 262,144 tokens are
+// 5e-5 short so, and were 1.75e-3 short without, seven times fp16's rounding.  A
+// total takes some 5 us of a CTA: 2,048 rows after 14,336, bf16 755 -> 770 us, and 790
+// with one every 4,096 tokens (2.6e-5).
+constexpr int kRunTokens = 8192;
 constexpr int kRing = 4;    // tiles whose exponent and token masks are kept
 
 template <int HD, int NQ, bool TWO>
 struct Pf {
     static constexpr int NT = HD == 256 ? 32 : 64;  // tokens of a tile
     static constexpr int NB = HD / 32;
+    static constexpr int kRun = kRunTokens / NT;  // tiles between rounded totals
     static constexpr int kParts = TWO ? 2 : 1;
     static constexpr int kQ = HD / 64 * kRows * 128;   // bytes of one part of one query tile
     static constexpr int kK = HD / 64 * NT * 128;      // keys: chunks of 64 dims, a row of 128 B per token
@@ -122,6 +130,9 @@ struct PfArgs {
     int q_tiles;   // CTAs along a sequence's rows
     uint32_t page_mul;
     int page_shift;
+    // half precision, contexts longer than kRunTokens: [kv head][chunk][hd][n_q * heads], so
+    // that a warp's rows, which follow one another, lie so in every column
+    float* totals;
 };
 
 // Instruction descriptors: both operands K-major, D f32.
@@ -154,6 +165,43 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 // 16-byte unit u (0..7) of row r of a 128-byte-swizzled tile
 __device__ __forceinline__ uint32_t sw128(int r, int u) { return (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4)); }
+
+// Half-precision queries: the outputs of a run of tiles (TMEM, this warp's lanes) go
+// to a row's totals, one for each column, `pairs` apart; `more`: on top of those
+// of the runs before, times `keep`.  (Functions of their own: inlined, they cost
+// the loop over the tiles its registers, 8% of the time.)
+template <int HD>
+__device__ __noinline__ void end_run(uint32_t o_at, float* total, int64_t pairs, bool more, float keep) {
+#pragma unroll 1
+    for (int j = 0; j < HD; j += 32) {
+        uint32_t o[32];
+        float y[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) y[k] = more && total ? total[(j + k) * pairs] : 0.0f;
+        tc::tmem_ld32(o_at + j, o);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+            if (total) total[(j + k) * pairs] = fmaf(y[k], keep, __uint_as_float(o[k]));
+    }
+}
+// And the totals, times `keep`, to the outputs of the last run.
+template <int HD>
+__device__ __noinline__ void add_runs(uint32_t o_at, const float* total, int64_t pairs, float keep) {
+#pragma unroll 1
+    for (int j = 0; j < HD; j += 32) {
+        uint32_t o[32];
+        float y[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) y[k] = total ? total[(j + k) * pairs] : 0.0f;
+        tc::tmem_ld32(o_at + j, o);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(y[k], keep, __uint_as_float(o[k])));
+        tc::tmem_st32(o_at + j, o);
+    }
+    tc::tmem_wait_st();
+}
 
 template <class T, int HD, int NQ>
 __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_q4_prefill_kernel(PfArgs p) {
@@ -306,7 +354,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                             for (int k = 0; k < NT / 8; ++k)
                                 mma_tf32_ts(d, t + part * C::kOffL + (i & 1) * NT + 8 * k,
                                             tc::sdesc_kmajor_sw128(vb + (k / 4) * HD * 128) + 2 * (k % 4), id,
-                                            (!kTwo && i) || part || k);
+                                            (!kTwo && i % C::kRun) || part || k);
                         commit(turn + 1 < kTurns ? t_part : o_done(q, i));
                     }
                     if (ok) commit(v_empty(i & 1));
@@ -534,7 +582,14 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         if (tiles) asm volatile("bar.arrive %0, 160;" ::"r"(1 + q_of) : "memory");
         const uint32_t tm = tmem + q_of * C::kCols + ((uint32_t)(warp % 4) << 21);  // this warp's 32 lanes
         const float c_row = a.scale * 1.44269504088896341f * pow2i(-q_exp[q_of * kRows + m_of]);
-        float m_run = -INFINITY, l = 0.0f;
+        float m_run = -INFINITY, l = 0.0f, m_total = -INFINITY;  // m_total: reference of the totals
+        const int64_t pairs = (int64_t)a.n_q * p.heads;
+        float* total = nullptr;
+        if constexpr (!kTwo)
+            if (my_row >= 0)
+                total = p.totals + (int64_t)(kvh * p.chunks + chunk) * HD * pairs + my_row * p.heads + m_of % nh;
+        // what moves the totals from their reference to m (a total without tokens is zeros)
+        auto total_factor = [&](float m) { return m_total == -INFINITY ? 0.0f : ex2(m_total - m); };
         uint32_t bad = 0;  // blocks of dimensions in which this row sees values that are not finite
         bool ok = true;
         auto wait = [&](uint32_t bar, int parity, int site) {
@@ -570,6 +625,14 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             return true;
         };
         for (int i = 0; ok && i < tiles; ++i) {
+            if (!kTwo && i && i % C::kRun == 0) {
+                // a run of tiles has ended: its outputs go to the totals, and the next
+                // one's start from zero
+                ok = wait(o_done(q_of, i - 1), (i - 1) >> 1, 53);
+                if (!ok) break;
+                end_run<HD>(tm + C::kOffO, total, pairs, i > C::kRun, total_factor(m_run));
+                m_total = m_run;
+            }
             ok = wait(s_full(q_of, i), i >> 1, 49);
             if (!ok) break;
             const uint32_t ts = tm + (i & 1) * NT;  // this tile's scores, and weights
@@ -644,7 +707,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             // the outputs up to the tile before, on the new reference
             if constexpr (kTwo)
                 if (i) ok = add_tile(i - 1);
-            if (ok && i && __any_sync(0xffffffffu, move)) {
+            if (ok && (kTwo ? i : i % C::kRun) && __any_sync(0xffffffffu, move)) {
                 if constexpr (!kTwo) ok = wait(o_done(q_of, i - 1), (i - 1) >> 1, 50);
 #pragma unroll 1
                 for (int j = 0; ok && j < HD / 32; ++j) {
@@ -667,6 +730,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             else ok = wait(o_done(q_of, tiles - 1), (tiles - 1) >> 1, 51);
         }
         if (ok) {
+            if (!kTwo && tiles > C::kRun) add_runs<HD>(tm + C::kOffO, total, pairs, total_factor(m_run));
             const float inv = l == 0.0f ? 0.0f : (kTwo ? kSumCut : kCut) / l;
             T* out = static_cast<T*>(a.out) + max(my_row, (int64_t)0) * (int64_t)a.out_stride + (int64_t)my_head * HD;
 #pragma unroll 1
@@ -741,8 +805,16 @@ cudaError_t attn_q4_prefill(int type, const AttnQ4Args& a, cudaStream_t s) {
     p.page_mul = (uint32_t)(((1ull << (31 + L)) + a.page - 1) / a.page);
     p.page_shift = L;
     if (type == kTypeF32) return prefill_of<float>(p, s);
-    if (type == kTypeF16) return prefill_of<__half>(p, s);
-    return prefill_of<__nv_bfloat16>(p, s);
+    if (a.max_ctx > kRunTokens) {
+        const uint64_t bytes = a.n_q * a.n_head_kv * p.chunks * p.heads * a.hd * sizeof(float);
+        if (cudaError_t e = scratch_alloc(reinterpret_cast<void**>(&p.totals), bytes, s)) return e;
+    }
+    cudaError_t e = type == kTypeF16 ? prefill_of<__half>(p, s) : prefill_of<__nv_bfloat16>(p, s);
+    if (p.totals) {
+        const cudaError_t f = cudaFreeAsync(p.totals, s);
+        if (e == cudaSuccess) e = f;
+    }
+    return e;
 }
 
 }  // namespace mvb

@@ -184,7 +184,8 @@ def one_sided(*args):
 
 
 def mean_off(got, q, ctx, t, kp, ks, vp, vs, page):
-    """Mean over the outputs of (got - want) / want; rows of one sequence."""
+    """Mean over the outputs of (got - want) / want, zeros for zeros apart; rows of
+    one sequence."""
     import torch
     rows, heads, hd = q.shape
     H, T = kp.shape[1], int(max(ctx))
@@ -197,7 +198,8 @@ def mean_off(got, q, ctx, t, kp, ks, vp, vs, page):
         v = values64(vp[pg, g], vs[pg, g]).reshape(-1, hd)[:T]
         s = (q[:, h].double() @ k.T * hd ** -0.5).masked_fill(past, -float("inf"))
         want = torch.softmax(s, -1) @ v
-        off.append(((got[:, h].double() - want) / want).mean())
+        assert not got[:, h][want == 0].any()
+        off.append(((got[:, h].double() - want) / torch.where(want == 0, 1.0, want)).mean())
     return float(torch.stack(off).mean())
 
 
@@ -214,6 +216,27 @@ def test_decode_long_half_sums_are_rounded(cuda, dtype, heads, hd):
     some = list(range(0, n, n // 50))
     noise = 1e-5 if dtype == "float16" else 4e-5  # of the outputs' rounding, over 50 x heads x hd outputs
     assert abs(mean_off(got[some], q[some], [T] * len(some), t, kp, ks, vp, vs, page)) <= 5e-5 + noise
+
+
+@pytest.mark.parametrize("dtype,heads,H,hd,rows", [("float16", 16, 8, 64, 150), ("float16", 8, 8, 128, 150),
+                                                   ("float16", 8, 4, 128, 2400), ("bfloat16", 8, 8, 128, 150),
+                                                   ("float16", 8, 8, 256, 150)])
+def test_prefill_long_half_sums_are_rounded(cuda, dtype, heads, H, hd, rows):
+    """Chunks at the end of 262,144 tokens (one and two query tiles to a CTA),
+    some rows ending far before."""
+    import torch
+    page, T = 128, 262_144
+    ctx = np.arange(T - rows + 1, T + 1, dtype=np.int32)
+    ctx[::7] = 1 + np.arange(len(ctx[::7])) * 761
+    t, kp, ks, vp, vs = one_sided(hd, H, T, page, 111)
+    q = randn((rows, heads, hd), 113, dtype, 0.5)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), T)
+    some = [r for r in range(0, rows, max(1, rows // 60)) if ctx[r] > T - rows]
+    noise = 1e-5 if dtype == "float16" else 4e-5
+    assert abs(mean_off(got[some], q[some], ctx[some], t, kp, ks, vp, vs, page)) <= 5e-5 + noise
+    some = list(range(0, rows, 7))[:40]
+    assert abs(mean_off(got[some], q[some], ctx[some], t, kp, ks, vp, vs, page)) <= 5e-5 + 2 * noise
+    assert torch.isfinite(got).all()
 
 
 # ------------------------------------------------------------------ scratch
