@@ -20,7 +20,8 @@
 // MMAs).  The tensor core cuts its running sums to 24 bits at every MMA instead
 // of rounding: summed over a whole context that takes 1.6e-8 an MMA off the
 // outputs (1.5e-4 after 32,768 tokens), so for fp32 queries a tile's outputs start
-// from zero and are added to the total, rounded, by the softmax warps.
+// from zero and are added to the total, rounded, by the softmax warps.  The second
+// parts go first: the sum is then 2^-11 of itself for half of its cuts.
 // A half-precision query is one part, and so are its weights, cut to 11 bits
 // by the tensor core, with 1 + 2^-11 0.72 on them for what that takes off on
 // average (mantissas being log-uniform).  Its outputs are summed by the tensor core
@@ -76,9 +77,6 @@ cudaError_t q4_status_take(int* status) {
 namespace {
 
 constexpr int kRows = 128;  // of a query tile: TMEM lanes
-// fp32: factor on the outputs for the 16 cut sums of a token tile's MMAs
-// (measured: they come out 1.0e-6 short, of 1.2e-6 in all).
-constexpr float kSumCut = 1.0f + 1.0f / 1048576;
 constexpr float kCutLog2 = 5.0811e-4f;  // log2(kCut)
 // Half-precision queries: tokens between rounded totals of the outputs, in scratch
 // (tensor memory is full).  Outputs of values of one sign after 262,144 tokens are
@@ -325,12 +323,13 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                     if (i >= 2 && !wait(o_done(q, i), (i - 2) >> 1, 41)) break;
                     const uint32_t kb = sb + C::kOffK + (i & 1) * C::kK, d = t + (i & 1) * NT;
 #pragma unroll
-                    for (int part = 0; part < C::kParts; ++part)
+                    for (int part = C::kParts - 1; part >= 0; --part)
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k)
                             mma_f16_ss(d,
                                        tc::sdesc_kmajor_sw128(qb + part * C::kQ + (k / 4) * kRows * 128) + 2 * (k % 4),
-                                       tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id, part || k);
+                                       tc::sdesc_kmajor_sw128(kb + (k / 4) * NT * 128) + 2 * (k % 4), id,
+                                       part + 1 < C::kParts || k);
                     commit(s_full(q, i));
                     if (lane == 0) tc::mbar_arrive(s_full(q, i));
                     commit(k_empty(i & 1));
@@ -349,12 +348,12 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                         const uint32_t vb = sb + C::kOffV + (i & 1) * C::kV + turn * C::OT * 128;
                         const uint32_t d = t + (kTwo ? C::kOffT : C::kOffO);
 #pragma unroll
-                        for (int part = 0; part < C::kParts; ++part)
+                        for (int part = C::kParts - 1; part >= 0; --part)
 #pragma unroll
                             for (int k = 0; k < NT / 8; ++k)
                                 mma_tf32_ts(d, t + part * C::kOffL + (i & 1) * NT + 8 * k,
                                             tc::sdesc_kmajor_sw128(vb + (k / 4) * HD * 128) + 2 * (k % 4), id,
-                                            (!kTwo && i % C::kRun) || part || k);
+                                            (!kTwo && i % C::kRun) || part + 1 < C::kParts || k);
                         commit(turn + 1 < kTurns ? t_part : o_done(q, i));
                     }
                     if (ok) commit(v_empty(i & 1));
@@ -731,7 +730,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         }
         if (ok) {
             if (!kTwo && tiles > C::kRun) add_runs<HD>(tm + C::kOffO, total, pairs, total_factor(m_run));
-            const float inv = l == 0.0f ? 0.0f : (kTwo ? kSumCut : kCut) / l;
+            const float inv = l == 0.0f ? 0.0f : (kTwo ? 1.0f : kCut) / l;
             T* out = static_cast<T*>(a.out) + max(my_row, (int64_t)0) * (int64_t)a.out_stride + (int64_t)my_head * HD;
 #pragma unroll 1
             for (int j = 0; j < HD / 32; ++j) {

@@ -239,6 +239,47 @@ def test_prefill_long_half_sums_are_rounded(cuda, dtype, heads, H, hd, rows):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("hd,H,heads", PROMPTS)
+def test_prefill_row_of_one_token_is_its_value(cuda, hd, H, heads):
+    """fp32 queries: the weight goes in as two parts of 11 bits (2^-22 of it may
+    be lost), their products' sum is cut once (2^-23), and divided by the weight;
+    three roundings."""
+    import torch
+    page, rows = 16, 150
+    t, total = scattered([rows], page, 114)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 115)
+    ctx = np.arange(1, rows + 1, dtype=np.int32)
+    ctx[::3] = 1
+    q = randn((rows, heads, hd), 116)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), rows)
+    want = values64(vp[int(t[0, 0]), :, 0], vs[int(t[0, 0]), :, 0]).repeat_interleave(heads // H, 0)
+    assert bool(((got[::3].double() - want).abs() <= (2.0 ** -22 + 2.0 ** -23 + 3 * 2.0 ** -24) * want.abs()).all())
+
+
+@pytest.mark.parametrize("hd,H,heads", PROMPTS)
+def test_prefill_long_fp32_sums_are_rounded(cuda, hd, H, heads):
+    """A tile's eight MMAs of first parts are cut (2^-24 of the sum each at most,
+    half of that on average, over the half of the tile's sum that is there on
+    average), its total is rounded; factors of 22 bits and the exponentials as
+    for decode steps: 1.2e-7 + 2.4e-7 + 2.4e-7, and as much again for scores."""
+    import torch
+    page, T, rows = 128, 30_000, 150
+    t, kp, ks, vp, vs = long_cache(hd, H, T, page, 117)
+    ctx = np.arange(T - rows + 1, T + 1, dtype=np.int32)
+    q = randn((rows, heads, hd), 119, "float32", 0.6)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), T).double()
+    pg = dev(t[0, :-(-T // page)].astype(np.int64))
+    past = torch.arange(T, device="cuda") >= dev(ctx)[:, None]
+    off = size = 0.0
+    for h in range(heads):
+        k, v = (values64(p[pg, h // (heads // H)], s[pg, h // (heads // H)]).reshape(-1, hd)[:T]
+                for p, s in ((kp, ks), (vp, vs)))
+        w = torch.softmax((q[:, h].double() @ k.T * hd ** -0.5).masked_fill(past, -float("inf")), -1) @ v
+        off += float(((got[:, h] - w) ** 2).sum())
+        size += float((w ** 2).sum())
+    assert (off / size) ** 0.5 <= 1.5e-6
+
+
 # ------------------------------------------------------------------ scratch
 
 @pytest.mark.parametrize("how", ["called", "captured first"])
