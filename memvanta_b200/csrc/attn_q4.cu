@@ -454,8 +454,9 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // times 2^e: the largest below 2^15
-        const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+        // times 2^e: the largest below 2^15, whatever its size (e > 100 would take the
+        // scores' factor out of range, and queries that small need no more bits)
+        const int e = min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127));
         const float up = pow2i(e);
         c_h = fmaxf(a.scale * 1.44269504088896341f * pow2i(-e), 1e-37f);
 #pragma unroll

@@ -552,8 +552,9 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                 }
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                // times 2^e: the largest below 2^15
-                const int e = max(-100, min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+                // times 2^e: the largest below 2^15, whatever its size (e > 100 would take the
+                // scores' factor out of range, and queries that small need no more bits)
+                const int e = min(100, 14 - ((int)(__float_as_uint(mx) >> 23) - 127));
                 const float up = pow2i(e);
                 if (u0 == 0) q_exp[q_of * kRows + m] = e;
 #pragma unroll

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import memvanta_b200 as mv
-from test_gpu_kv_q4 import attention64, check_attention, randn, random_cache, scattered, values64
+from test_gpu_kv_q4 import attention64, check_attention, randn, random_cache, scattered, tdtype, values64
 
 pytestmark = pytest.mark.gpu
 TYPES = ["float32", "float16", "bfloat16"]
@@ -278,6 +278,44 @@ def test_prefill_long_fp32_sums_are_rounded(cuda, hd, H, heads):
         off += float(((got[:, h] - w) ** 2).sum())
         size += float((w ** 2).sum())
     assert (off / size) ** 0.5 <= 1.5e-6
+
+
+# ---------------------------------------------------------- queries of any size
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("e", [116, 90, -90])
+def test_queries_of_any_size(cuda, dtype, e):
+    """Queries of 2^e over keys of 2^-e: scores as of 1 over 1."""
+    import torch
+    heads, H, hd, page, T, rows = 8, 8, 128, 16, 200, 150
+    t, total = scattered([T], page, 120)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 121)
+    ks = (ks.double() * 2.0 ** -e).bfloat16()
+    q = (randn((rows, heads, hd), 122, dtype).double() * 2.0 ** e).to(tdtype(dtype))
+    ctx = np.arange(T - rows + 1, T + 1, dtype=np.int32)
+    want, bound = attention64(q, kp, ks, vp, vs, t, [0] * rows, ctx, page, hd ** -0.5)
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), T)
+    check_attention(got, want, bound)
+    got = mv.paged_attn_q4(q, kp, vp, ks, vs, dev(np.repeat(t, rows, 0)), dev(ctx), T)
+    check_attention(got, want, bound)
+
+
+def test_decode_value_scales_that_grow_along_the_context(cuda):
+    """By 2^40 from the first token to the last, and the other way round."""
+    import torch
+    heads, H, hd, page, ctx = 4, 2, 64, 16, 1000
+    t, total = scattered([ctx], page, 123)
+    kp, ks, vp, vs = random_cache(total, H, page, hd, 124)
+    q = randn((1, heads, hd), 125)
+    for a, b in ((-20, 20), (20, -20)):
+        grow = torch.ones((total, page), dtype=torch.float64, device=cuda)
+        pages = -(-ctx // page)
+        grow[dev(t[0, :pages].astype(np.int64))] = 2.0 ** torch.linspace(a, b, pages * page, dtype=torch.float64,
+                                                                       device=cuda).view(pages, page)
+        vs2 = (vs.double() * grow[:, None, :, None]).bfloat16()
+        got = mv.paged_attn_q4(q, kp, vp, ks, vs2, dev(t), i32([ctx]), ctx)
+        want, bound = attention64(q, kp, ks, vp, vs2, t, [0], [ctx], page, hd ** -0.5)
+        check_attention(got, want, bound)
 
 
 # ------------------------------------------------------------------ scratch
