@@ -318,9 +318,10 @@ MV_API int mv_kv_read(int kv_type, const void* pages_dev, const void* scales_dev
  * max_ctx (and max_pages*page); a row with no tokens gives zeros; tokens on a page
  * outside [0, n_pages) are left out.  Scores, sums and outputs are held in fp32; for
  * F32 queries the products carry 22 bits of each factor, for F16 and BF16
- * queries the queries' own.  Queries may have any size, cached keys and values up
- * to 2^80 (sums of values times 16^3 are held in fp32).  Scratch is stream-ordered and comes from a pool of
- * the library's own, which keeps it; calls may be captured in graphs. */
+ * queries the queries' own and weights rounded to 11 bits.  Queries may have any
+ * size, cached keys and values up to 2^80 (sums of values times 16^3 are held in
+ * fp32).  Scratch is stream-ordered and comes from a pool of the library's own,
+ * which keeps it; calls may be captured in graphs. */
 MV_API int mv_paged_attn_q4(int type, const void* q_dev, uint64_t q_row_stride, uint64_t n_seq, uint64_t n_head,
                             uint64_t n_head_kv, uint64_t head_dim, const void* k_pages_dev, const void* v_pages_dev,
                             const void* k_scales_dev, const void* v_scales_dev, const int32_t* block_table_dev,

@@ -100,8 +100,7 @@ __device__ __forceinline__ void mma1688(float (&d)[4], const float (&a)[4], floa
 // four heads (PACK: rows 4..7 repeat heads 0..3, so a lane's weights are
 // already there) and a second MMA for more.  The tensor core ignores the low
 // 13 bits of a tf32 operand, so the first part needs no masking; half-precision
-// queries' weights go in as one part, and p carries a factor kCut that makes up
-// for what that cut takes off on average.
+// queries' weights go in as one part, rounded to 11 bits.
 constexpr int kWarps = 4, kStages = 3;
 constexpr int kShort = 8;  // stages to a warp of a cluster at most
 
@@ -592,7 +591,6 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
                     for (int i = 0; i < 2; ++i) {
                         p[i] = ex2(fmaf(sc[j][i], c_h, -m_use));
                         l_run += p[i];
-                        if constexpr (!kTwo) p[i] *= kCut;
                         load_words<HD>(w[i], vt, 8 * j + 2 * t + i, g >> 1);
                     }
                     const uint64_t pp = pair(p[0], p[1]);
@@ -601,6 +599,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 ? 3 : 2) attn_q4_decode
                         float v[2];
                         const uint64_t vv = tc::f2_mul(pp, pair(scale_of<HD>(d, 0, b), scale_of<HD>(d, 1, b)));
                         unpair(vv, v[0], v[1]);
+                        if constexpr (!kTwo) v[0] = near11(v[0]), v[1] = near11(v[1]);
                         const uint32_t x0 = w[0][b] >> half, x1 = w[1][b] >> half;
                         float f0[4], f1[4];  // rows g, g + 8 of the first token, then of the second
                         values2<0>(x0, bias0, f0[0], f0[1]);

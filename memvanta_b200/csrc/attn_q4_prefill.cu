@@ -22,10 +22,10 @@
 // outputs (1.5e-4 after 32,768 tokens), so for fp32 queries a tile's outputs start
 // from zero and are added to the total, rounded, by the softmax warps.  The second
 // parts go first: the sum is then 2^-11 of itself for half of its cuts.
-// A half-precision query is one part, and so are its weights, cut to 11 bits
-// by the tensor core, with 1 + 2^-11 0.72 on them for what that takes off on
-// average (mantissas being log-uniform).  Its outputs are summed by the tensor core
-// for kRunTokens tokens at a time.
+// A half-precision query is one part, and so are its weights, rounded to 11 bits
+// (rounded here, since the tensor core cuts: 764 -> 782 us for the 2,048 rows below;
+// with the sum of the rounded weights below the line too, 796 us).  Its outputs are
+// summed by the tensor core for kRunTokens tokens at a time.
 // A masked weight is 0, and 0 times a value that is not finite would not be: such
 // value blocks enter as zeros, and the rows that see one get NaN in its
 // dimensions at the end.
@@ -77,7 +77,6 @@ cudaError_t q4_status_take(int* status) {
 namespace {
 
 constexpr int kRows = 128;  // of a query tile: TMEM lanes
-constexpr float kCutLog2 = 5.0811e-4f;  // log2(kCut)
 // Half-precision queries: tokens between rounded totals of the outputs, in scratch
 // (tensor memory is full).  Outputs of values of one sign after 262,144 tokens are
 // 5e-5 short so, and were 1.75e-3 short without, seven times fp16's rounding.  A
@@ -678,7 +677,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
             const float alpha = move ? ex2(m_run - mx) : 1.0f;
             if (move) m_run = mx;
             l *= alpha;
-            const float m_use = (m_run == -INFINITY ? 0.0f : m_run) - (kTwo ? 0.0f : kCutLog2);
+            const float m_use = m_run == -INFINITY ? 0.0f : m_run;
             const uint64_t cc = pair(c, c), mm = pair(-m_use, -m_use);
             uint64_t l2[2] = {0, 0};
 #pragma unroll
@@ -691,6 +690,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
                     unpair(tc::f2_fma(pair(__uint_as_float(sp[0]), __uint_as_float(sp[1])), cc, mm), x0, x1);
                     x0 = ex2(x0), x1 = ex2(x1);
                     l2[k / 2 % 2] = f2_add(l2[k / 2 % 2], pair(x0, x1));
+                    if constexpr (!kTwo) x0 = near11(x0), x1 = near11(x1);
                     w[k] = __float_as_uint(x0), w[k + 1] = __float_as_uint(x1);
                     if constexpr (kTwo) {
                         w[k] &= 0xffffe000u, w[k + 1] &= 0xffffe000u;  // 11 bits
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(Pf<HD, NQ, sizeof(T) == 4>::kThreads, 1) attn_
         }
         if (ok) {
             if (!kTwo && tiles > C::kRun) add_runs<HD>(tm + C::kOffO, total, pairs, total_factor(m_run));
-            const float inv = l == 0.0f ? 0.0f : (kTwo ? 1.0f : kCut) / l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T* out = static_cast<T*>(a.out) + max(my_row, (int64_t)0) * (int64_t)a.out_stride + (int64_t)my_head * HD;
 #pragma unroll 1
             for (int j = 0; j < HD / 32; ++j) {

@@ -205,10 +205,9 @@ __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t* 
 }
 
 // ------------------------------------------------- arithmetic on the blocks
-// Half-precision queries: factor on the weights for what their cut to 11 bits
-// (tf32, by the tensor core) takes off on average, 1 + 2^-11 / (2 ln 2), their
-// mantissas being log-uniform.
-constexpr float kCut = 1.00035225f;
+// Half-precision queries: a weight such that its first 11 bits, which are what the
+// tensor core takes of a tf32 operand, are the nearest 11 (ties away from zero).
+__device__ __forceinline__ float near11(float x) { return __uint_as_float(__float_as_uint(x) + 0x1000u); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import memvanta_b200 as mv
-from test_gpu_kv_q4 import attention64, check_attention, randn, random_cache, scattered, tdtype, values64
+from test_gpu_kv_q4 import attention64, check_attention, layout_index, randn, random_cache, scattered, tdtype, values64
 
 pytestmark = pytest.mark.gpu
 TYPES = ["float32", "float16", "bfloat16"]
@@ -237,6 +237,41 @@ def test_prefill_long_half_sums_are_rounded(cuda, dtype, heads, H, hd, rows):
     some = list(range(0, rows, 7))[:40]
     assert abs(mean_off(got[some], q[some], ctx[some], t, kp, ks, vp, vs, page)) <= 5e-5 + 2 * noise
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("route", ["decode", "prompt"])
+@pytest.mark.parametrize("x0", [7.0, 7.875])
+def test_half_weights_are_rounded_not_cut(cuda, route, x0):
+    """64 tokens of score 0 and value 0, then one whose weight 2^x is just above, or
+    just below, a power of two: outputs w v / (64 + 2^x), w of 11 bits.  Rounded, w
+    is off by at most 2^-11 either way, which leaves nothing in the mean over 1,776
+    rows (a hundred steps of w) and 7 values; the outputs' rounding leaves 2e-6."""
+    import torch
+    n, hd, page, T, heads = 1776, 64, 128, 65, 1
+    kp, vp = (torch.full((1, 1, page, hd // 2), 0x88, dtype=torch.uint8, device=cuda) for _ in range(2))
+    ks, vs = (torch.zeros((1, 1, page, hd // 32), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    ks[0, 0, 64] = vs[0, 0, 64] = 1
+    kp[0, 0, 64, 0] = 0x99  # dimensions 0 and 1: 1, the others 0
+    values = 1 + torch.arange(hd, device=cuda) % 7
+    byte, shift = layout_index(hd)
+    vp[0, 0, 64] = 0
+    vp[0, 0, 64].index_add_(0, dev(byte).long(), ((values + 8) << dev(shift)).to(torch.uint8))
+    assert torch.equal(values64(vp, vs)[0, 0, 64], values.double())
+    q = torch.zeros((n, heads, hd), dtype=torch.float16, device=cuda)
+    q[:, 0, 0] = x0
+    q[:, 0, 1] = torch.arange(n, device=cuda) * ((0.1375 if x0 == 7 else 0.09) / n)
+    scale = float(np.float32(np.log(2)))
+    pages = (kp, vp, ks, vs)
+    if route == "decode":
+        got = mv.paged_attn_q4(q, *pages, torch.zeros((n, 1), dtype=torch.int32, device=cuda), i32([T] * n), T, scale)
+    else:
+        got = mv.paged_attn_q4_prefill(q, *pages, torch.zeros((1, 1), dtype=torch.int32, device=cuda), i32([0, n]), n,
+                                       i32([T] * n), T, scale)
+    p = torch.exp(scale * (q[:, 0, 0].double() + q[:, 0, 1].double()))[:, None]
+    want = p * values / (64 + p)
+    off = got[:, 0].double() / want - 1
+    assert float(off.abs().max()) <= 2.0 ** -11 + 2.0 ** -11 + 2e-6
+    assert abs(float(off.mean())) <= 2e-5
 
 
 @pytest.mark.parametrize("hd,H,heads", PROMPTS)
