@@ -1151,20 +1151,27 @@ void load_model(mv_model_s* m, const char* path, uint64_t ctx, uint64_t page, in
         L.k_scales = ns ? dalloc<float>(m, rows * ns) : nullptr;
         L.v_scales = ns ? dalloc<float>(m, rows * ns) : nullptr;
     }
-    // RoPE tables exactly as the reference builds them (src/llama_model.cpp:233)
     const uint64_t half = m->hd / 2;
-    std::vector<float> co(m->n_ctx * half), si(m->n_ctx * half);
-    for (uint64_t p = 0; p < m->n_ctx; ++p)
-        for (uint64_t i = 0; i < half; ++i) {
-            const float inv = std::pow(m->theta, -2.0f * float(i) / float(m->hd));
-            const float a = float(p) * inv;
-            co[p * half + i] = std::cos(a);
-            si[p * half + i] = std::sin(a);
-        }
-    m->rope_cos = dalloc<float>(m, co.size());
-    m->rope_sin = dalloc<float>(m, si.size());
-    ck(cudaMemcpy(m->rope_cos, co.data(), co.size() * 4, cudaMemcpyHostToDevice), "rope cos");
-    ck(cudaMemcpy(m->rope_sin, si.data(), si.size() * 4, cudaMemcpyHostToDevice), "rope sin");
+    m->rope_cos = dalloc<float>(m, m->n_ctx * half);
+    m->rope_sin = dalloc<float>(m, m->n_ctx * half);
+    if (kv_type == MV_KV_Q4_0) {
+        // angles in double: the reference's are off by up to 2^-8 at position 131,071
+        ck(mvb::rope_table({MV_ROPE_SCALE_NONE, m->theta}, m->hd, m->n_ctx, nullptr, m->rope_cos, m->rope_sin, 0),
+           "rope tables");
+        ck(cudaStreamSynchronize(0), "rope tables");
+    } else {
+        // exactly as the reference builds them (src/llama_model.cpp:233)
+        std::vector<float> co(m->n_ctx * half), si(m->n_ctx * half);
+        for (uint64_t p = 0; p < m->n_ctx; ++p)
+            for (uint64_t i = 0; i < half; ++i) {
+                const float inv = std::pow(m->theta, -2.0f * float(i) / float(m->hd));
+                const float a = float(p) * inv;
+                co[p * half + i] = std::cos(a);
+                si[p * half + i] = std::sin(a);
+            }
+        ck(cudaMemcpy(m->rope_cos, co.data(), co.size() * 4, cudaMemcpyHostToDevice), "rope cos");
+        ck(cudaMemcpy(m->rope_sin, si.data(), si.size() * 4, cudaMemcpyHostToDevice), "rope sin");
+    }
 
     const uint64_t D = m->n_embd, F = m->n_ff;
     if (world > 1) {
