@@ -203,6 +203,34 @@ def mean_off(got, q, ctx, t, kp, ks, vp, vs, page):
     return float(torch.stack(off).mean())
 
 
+def far_off(got, q, ctx, t, kp, ks, vp, vs, page):
+    """Relative error of the outputs, root mean square; rows of one sequence."""
+    import torch
+    heads, hd, H, T = q.shape[1], q.shape[2], kp.shape[1], int(max(ctx))
+    pg = dev(t[0, :-(-T // page)].astype(np.int64))
+    past = torch.arange(T, device="cuda") >= i32(list(ctx))[:, None]
+    off = size = 0.0
+    for h in range(heads):
+        k, v = (values64(p[pg, h // (heads // H)], s[pg, h // (heads // H)]).reshape(-1, hd)[:T]
+                for p, s in ((kp, ks), (vp, vs)))
+        w = torch.softmax((q[:, h].double() @ k.T * hd ** -0.5).masked_fill(past, -float("inf")), -1) @ v
+        off += float(((got[:, h].double() - w) ** 2).sum())
+        size += float((w ** 2).sum())
+    return (off / size) ** 0.5
+
+
+@pytest.mark.parametrize("H,heads,hd,n,T", [(1, 8, 64, 3, 90_001), (4, 4, 64, 1, 700), (2, 16, 256, 2, 40_003),
+                                            (8, 8, 256, 20, 3000), (8, 56, 128, 2, 30_011), (8, 32, 128, 64, 2000)])
+def test_decode_fp32_loses_no_bits(cuda, H, heads, hd, n, T):
+    """As test_decode_long_sums_are_rounded, and with its bound, whatever the group,
+    the head size, the route and the length."""
+    page = 128
+    t, kp, ks, vp, vs = long_cache(hd, H, T, page, 126)
+    q = randn((n, heads, hd), 128, "float32", 0.6)
+    got = mv.paged_attn_q4(q, kp, vp, ks, vs, dev(np.repeat(t, n, 0)), i32([T] * n), T)
+    assert far_off(got, q, [T] * n, t, kp, ks, vp, vs, page) <= 1.5e-6
+
+
 @pytest.mark.parametrize("dtype,heads,hd", [("float16", 8, 128), ("float16", 8, 64), ("bfloat16", 2, 128),
                                             ("float16", 2, 256)])
 def test_decode_long_half_sums_are_rounded(cuda, dtype, heads, hd):
@@ -302,17 +330,8 @@ def test_prefill_long_fp32_sums_are_rounded(cuda, hd, H, heads):
     t, kp, ks, vp, vs = long_cache(hd, H, T, page, 117)
     ctx = np.arange(T - rows + 1, T + 1, dtype=np.int32)
     q = randn((rows, heads, hd), 119, "float32", 0.6)
-    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), T).double()
-    pg = dev(t[0, :-(-T // page)].astype(np.int64))
-    past = torch.arange(T, device="cuda") >= dev(ctx)[:, None]
-    off = size = 0.0
-    for h in range(heads):
-        k, v = (values64(p[pg, h // (heads // H)], s[pg, h // (heads // H)]).reshape(-1, hd)[:T]
-                for p, s in ((kp, ks), (vp, vs)))
-        w = torch.softmax((q[:, h].double() @ k.T * hd ** -0.5).masked_fill(past, -float("inf")), -1) @ v
-        off += float(((got[:, h] - w) ** 2).sum())
-        size += float((w ** 2).sum())
-    assert (off / size) ** 0.5 <= 1.5e-6
+    got = mv.paged_attn_q4_prefill(q, kp, vp, ks, vs, dev(t), i32([0, rows]), rows, dev(ctx), T)
+    assert far_off(got, q, ctx, t, kp, ks, vp, vs, page) <= 1.5e-6
 
 
 # ---------------------------------------------------------- queries of any size
