@@ -290,7 +290,7 @@ MV_API int mv_rope_apply(int type, const void* x_dev, uint64_t x_row_stride, uin
  * holds dimensions 32b+8t .. +7, lowest nibble first.  A block of 32: mx its
  * element of largest magnitude (first of equals), d = bf16(mx/-8), n =
  * clamp(floor(x*(1/d) + 8.5), 0, 15), value (n-8)*d; a block with a NaN or
- * infinity reads back as NaN.
+ * infinity reads back as NaN, one whose largest magnitude is below 2^-100 as zeros.
  * Replaces mv_rope + mv_kv_append (src/llama_model.cpp:238, :22). */
 MV_API int mv_rope_kv_append(int kv_type, int type, const void* q_dev, uint64_t q_row_stride, uint64_t q_head_stride,
                              void* q_out_dev, uint64_t q_out_row_stride, uint64_t q_out_head_stride, uint64_t n_head,
@@ -331,7 +331,8 @@ MV_API int mv_paged_attn_q4(int type, const void* q_dev, uint64_t q_row_stride, 
  * q_start[s+1] of the n_q rows (device array of n_seq + 1, ascending from 0 to
  * n_q), at most max_q of them; row r attends to its first ctx_len[r] tokens
  * (causal: start + i + 1).  Rows of no sequence, and a sequence's rows past its
- * first max_q, give zeros. */
+ * first max_q, give zeros.  F16 and BF16 queries with max_ctx above 8192 take
+ * n_q * n_head * head_dim * 4 bytes of scratch. */
 MV_API int mv_paged_attn_q4_prefill(int type, const void* q_dev, uint64_t q_row_stride, uint64_t n_q, uint64_t n_head,
                                     uint64_t n_head_kv, uint64_t head_dim, const void* k_pages_dev,
                                     const void* v_pages_dev, const void* k_scales_dev, const void* v_scales_dev,

@@ -6,13 +6,14 @@
 // lies past ctx_len, or on a page that does not exist, is never used.
 //
 // Measured (back-to-back launches; 2 x (hd / 2 + hd / 16) bytes a token and kv head):
-//   1 x 768 tokens, 32 kv heads x 128, fp32 queries          6.6 us  (latency)
-//   1 x 131,071 tokens, 8 kv heads x 128, 32 heads fp32      59.5 us  151 MB: 2.5 TB/s, 0.39 of HBM's
+//   1 x 768 tokens, 32 kv heads x 128, fp32 queries          6.7 us  (latency)
+//   1 x 131,071 tokens, 8 kv heads x 128, 32 heads fp32      59.1 us  151 MB: 2.6 TB/s, 0.39 of HBM's
 //   64 x 64..768 tokens, 32 heads x 128 fp32                 48.3 us  1.9 TB/s
-//   48 x 1..16,384 tokens, 8 kv heads x 64, 64 heads fp16    66.4 us  2.3 TB/s
+//   48 x 1..16,384 tokens, 8 kv heads x 64, 64 heads fp16    66.8 us  2.3 TB/s
+//   64 x 2,000 tokens, 4 kv heads x 256, 16 heads bf16       66.4 us  2.2 TB/s
 // Long contexts are bound by instructions -- some 440 for 16 tokens of head_dim 128, half
 // of the integer pipe's time, a third of the tensor cores' -- and not by memory:
-// the same ring without its arithmetic takes 24.5 us for the 59.5.
+// the same ring without its arithmetic takes 24.5 us for the 59.1.
 // Tried: two stages to a ring, 80 to 96 registers, more and smaller CTAs (slower).
 #include <cuda_runtime.h>
 
@@ -950,8 +951,9 @@ cudaError_t decode_of(int type, const AttnQ4Args& a, cudaStream_t s, uint64_t* n
 // kv head costs it 46 to 57 ps a token (head_dim 128, fp32), whereas a wave of the
 // tensor-core kernel's CTAs takes 25 ns a token however few of its 128 rows are
 // used -- as much as 550 rows.  Measured by head_dim 64, 128, 256: 820, 550, 770 rows
-// (fp32 queries), 640, 415, 440 (half precision).  The bounds lie below all of them,
-// since a causal chunk's first rows are cheap for both and its tiles are not.
+// (fp32 queries; 700, 490, 700 for groups above 4), 640, 425, 450 (half precision).
+// The bounds are set low, since a causal chunk's first rows are cheap row by row and
+// its tiles are not.
 // Only the tiles that hold rows count, each sequence's last one part empty; a CTA
 // without rows leaves its SM after 1.1 us, a wave's 25 ns for 44 tokens.  One chunk of
 // 2,048 rows and 63 single rows after 700 tokens, 32 heads x 128: fp32 775 us (row by

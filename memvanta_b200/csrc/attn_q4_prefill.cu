@@ -23,8 +23,8 @@
 // from zero and are added to the total, rounded, by the softmax warps.  The second
 // parts go first: the sum is then 2^-11 of itself for half of its cuts.
 // A half-precision query is one part, and so are its weights, rounded to 11 bits
-// (rounded here, since the tensor core cuts: 764 -> 782 us for the 2,048 rows below;
-// with the sum of the rounded weights below the line too, 796 us).  Its outputs are
+// (rounded here, since the tensor core cuts: 764 -> 782 us for 2,048 rows at 16,384
+// tokens; divided by the sum of the rounded weights, 796 us).  Its outputs are
 // summed by the tensor core for kRunTokens tokens at a time.
 // A masked weight is 0, and 0 times a value that is not finite would not be: such
 // value blocks enter as zeros, and the rows that see one get NaN in its
@@ -38,17 +38,18 @@
 // SM a CTA.  The last query tiles start first: they see the most tokens.
 // Measured (back-to-back launches):
 //   512 rows, 32 heads x 128, fp32                          24.4 us
-//   2,048 rows after 14,336, 32 heads / 8 x 128, bf16        690 us  515 GFLOP: 0.75 PFLOP/s, 0.45 of bf16
+//   2,048 rows after 14,336, 32 heads / 8 x 128, bf16        726 us  515 GFLOP: 0.71 PFLOP/s, 0.43 of bf16
 //   7 x 331 rows after 1,500, 16 heads / 4 x 256, fp16       88 us  0.21 PFLOP/s
-// Bound by latency: per token tile 1.57 us (fp32), 1.12 us (half precision, head_dim
-// 128; two query tiles 2.7 us), 2.5 us (head_dim 256, 32 tokens twice), of which the
+// Bound by latency: per token tile 1.65 us (fp32), 1.17 us (half precision, head_dim
+// 128; two query tiles 3.0 us), 2.5 us (head_dim 256, 32 tokens twice), of which the
 // MMAs take 0.5 to 0.6 us a query tile; the rest is the chain scores - maximum -
 // weights - outputs of 64 exponentials a thread and the hand-offs.  9 us (fp32) or
 // 6 us (half) are launch, queries, first tile and outputs; and the last wave of
 // CTAs is part empty (256 CTAs and 308 on 148 SMs).
-// Tried: one warp issuing all MMAs in order (870 us for the 690), one lane polling
-// for its warp (+8%), a single buffer of scores (fp32 +13%), outputs through shared
-// memory in whole lines (1 us less at the end, 4% more in the loop: registers).
+// Tried (when the 2,048 rows took 690 us): one warp issuing all MMAs in order (870
+// us), one lane polling for its warp (+8%), a single buffer of scores (fp32 +13%),
+// outputs through shared memory in whole lines (1 us less at the end, 4% more in
+// the loop: registers).
 #include <cuda_runtime.h>
 
 #include <algorithm>

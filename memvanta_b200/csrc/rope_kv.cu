@@ -17,8 +17,9 @@
 //   reading 4,093 rows x 32 x 128 of Q4_0 back as fp16         10.9 us  4.0 TB/s
 // The Q4_0 append is bound by instructions: 500 for 16 dimensions of K and V, half
 // of them the block's scale and the rounding of its nibbles (63% of the issue
-// slots are taken, 36% of the memory's time).  Small calls are a launch and three
-// loads that wait on one another (position, page, angle).
+// slots are taken, 36% of the memory's time).  So is the read-back: 16 instructions
+// a value, 75% of the issue slots, 64% of the integer pipe.  Small calls are a
+// launch and three loads that wait on one another (position, page, angle).
 // Tried: a thread for several heads, so that the row's part is done once
 // (113 to 127 us with its reads, 101 without: fewer threads hide less), lines
 // asked for into L2 a wave ahead (no change), 8-byte accesses for half types
